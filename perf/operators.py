@@ -1,0 +1,318 @@
+"""The 8-bit first stage of a retrieval and the loss that trains its encoder, as measured work.
+
+Four operators, each reached through the package's device entries:
+  norm      an encoder's last step: residual addition, root-mean-square norm, rows of 8-bit integers with a scale
+  quantize  rows as they are (a corpus, an encoder's finished vectors) to 8-bit integers with a scale
+  product   8-bit rows against 8-bit rows, each with its scale: scores of queries over a corpus, or a linear layer
+  distill   Kullback-Leibler loss of a row of logits against a teacher's best k (what an exact search returns), and its gradient
+
+`run` computes them as plain torch operations, or (own = True) with the package's kernels.
+"""
+import importlib.util
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+_SIZE = {"f32": 4, "f16": 2, "bf16": 2}
+_CODE = {"f32": 0, "f16": 1, "bf16": 2}
+_EPS = 1e-6
+
+
+def listed():
+    return [
+        # one token of a served encoder: the call's latency counts
+        {"name": "norm_token", "op": "norm", "dtype": "bf16", "rows": 1, "dim": 4096, "pad": 0, "residual": True},
+        # a ragged batch of odd width, rows cut out of a wider buffer, single precision
+        {"name": "norm_ragged", "op": "norm", "dtype": "f32", "rows": 1531, "dim": 1021, "pad": 14, "residual": True},
+        # a large prompt batch
+        {"name": "norm_prompt", "op": "norm", "dtype": "bf16", "rows": 16384, "dim": 4096, "pad": 0, "residual": True},
+        # a batch of finished sentence vectors on its way into an index
+        {"name": "quantize_batch", "op": "quantize", "dtype": "f16", "rows": 1000, "dim": 768, "pad": 0},
+        # an index of a million single-precision rows built in one call
+        {"name": "quantize_corpus", "op": "quantize", "dtype": "f32", "rows": 1_000_000, "dim": 384, "pad": 0},
+        # one query over a million rows
+        {"name": "product_query", "op": "product", "to": "f32", "m": 1, "n": 1_000_000, "dim": 384, "pad": 0},
+        # a decoding step's linear layer for a small batch
+        {"name": "product_decode", "op": "product", "to": "bf16", "m": 16, "n": 4096, "dim": 4096, "pad": 0},
+        # an odd number of queries over odd rows at odd strides
+        {"name": "product_odd", "op": "product", "to": "f16", "m": 37, "n": 50021, "dim": 777, "pad": 3},
+        # a prompt's linear layer: the matrix cores' own rate
+        {"name": "product_prompt", "op": "product", "to": "bf16", "m": 4096, "n": 16384, "dim": 4096, "pad": 0},
+        # evaluation of 64 queries' scores over a million rows, no gradient
+        {"name": "distill_eval", "op": "distill", "what": "loss", "dtype": "f32", "rows": 64, "cols": 1_000_000, "k": 100, "pad": 0},
+        # a training step: loss and gradient together
+        {"name": "distill_step", "op": "distill", "what": "step", "dtype": "bf16", "rows": 4096, "cols": 32000, "k": 64, "pad": 0},
+        # the gradient alone, from the saved normaliser, for a few rows of odd length
+        {"name": "distill_grad", "op": "distill", "what": "grad", "dtype": "f16", "rows": 50, "cols": 10007, "k": 10, "pad": 5},
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(["norm", "quantize", "product", "product", "distill", "distill"])
+    pad = rng.choice([0, 0, 0, rng.randint(1, 40)])
+    if op == "norm":
+        dim = _log(rng, 33, 12288)
+        if rng.random() < 0.6:
+            dim = max(64, dim // 64 * 64)
+        rows = _log(rng, 1, min(16384, 60_000_000 // dim))
+        return {"op": op, "dtype": rng.choice(["f32", "f16", "bf16", "bf16"]), "rows": rows, "dim": dim, "pad": pad, "residual": rng.random() < 0.7}
+    if op == "quantize":
+        dim = _log(rng, 16, 4096)
+        if rng.random() < 0.6:
+            dim = max(64, dim // 64 * 64)
+        rows = _log(rng, 1, min(1_000_000, 300_000_000 // dim))
+        return {"op": op, "dtype": rng.choice(["f32", "f32", "f16", "bf16"]), "rows": rows, "dim": dim, "pad": pad}
+    if op == "product":
+        dim = _log(rng, 32, 8192)
+        if rng.random() < 0.7:
+            dim = max(64, dim // 64 * 64)
+        m = _log(rng, 1, 4096)
+        n = _log(rng, 64, min(1_000_000, 300_000_000 // dim, 60_000_000 // m))
+        return {"op": op, "to": rng.choice(["f32", "f16", "bf16", "bf16"]), "m": m, "n": n, "dim": dim, "pad": pad}
+    cols = _log(rng, 100, 1_000_000)
+    rows = _log(rng, 1, min(4096, 60_000_000 // cols))
+    return {"op": op, "what": rng.choice(["loss", "step", "step", "grad"]), "dtype": rng.choice(["f32", "f16", "bf16", "bf16"]),
+            "rows": rows, "cols": cols, "k": rng.randint(1, min(128, cols)), "pad": pad}
+
+
+def _strided(rows, cols, pad, dtype):
+    """An empty (rows, cols) tensor whose rows lie cols + pad apart."""
+    return torch.empty((rows, cols + pad), dtype=dtype, device="cuda")[:, :cols]
+
+
+def _filled(values, pad):
+    if not pad:
+        return values.contiguous()
+    t = _strided(values.shape[0], values.shape[1], pad, values.dtype)
+    t.copy_(values)
+    return t
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+
+    def normal(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    op, s = case["op"], dict(case)
+    if op in ("norm", "quantize"):
+        t, rows, dim, pad = _TYPES[case["dtype"]], case["rows"], case["dim"], case["pad"]
+        # hidden states: token sizes differ, a few channels stand out
+        channel = torch.exp(0.5 * normal(dim))
+        s["x"] = _filled((normal(rows, dim) * channel * torch.exp(0.3 * normal(rows, 1))).to(t), pad)
+        if op == "norm":
+            s["residual_in"] = _filled((normal(rows, dim) * channel).to(t), pad) if case["residual"] else None
+            s["weight"] = (1 + 0.1 * normal(dim)).to(t)
+            s["sum"] = _strided(rows, dim, pad, t)
+        s["q8"] = torch.empty((rows, dim), dtype=torch.int8, device="cuda")
+        s["scale"] = torch.empty(rows, dtype=torch.float32, device="cuda")
+        s["values"] = _strided(rows, dim, pad, t)
+    elif op == "product":
+        m, n, dim, pad = case["m"], case["n"], case["dim"], case["pad"]
+
+        def rows8(count):
+            # what 8-bit rows look like: normal components, the largest of a row at 127
+            return _filled((normal(count, dim) * 32).round_().clamp_(-127, 127).to(torch.int8), pad)
+
+        s["a"], s["b"] = rows8(m), rows8(n)
+        s["a_scale"] = torch.exp(0.3 * normal(m)) / 32
+        s["b_scale"] = torch.exp(0.3 * normal(n)) / (32 * math.sqrt(dim))
+        s["out"] = torch.empty((m, n), dtype=_TYPES[case["to"]], device="cuda")
+    else:
+        t, rows, cols, k, pad = _TYPES[case["dtype"]], case["rows"], case["cols"], case["k"], case["pad"]
+        logits = _filled((2 * normal(rows, cols)).to(t), pad)
+        s["logits"] = logits
+        # a teacher's list: k different columns, best first, some lists shorter than k, now and then an empty one
+        start = torch.randint(0, cols, (rows, 1), generator=g, device="cuda")
+        step = max(1, cols // (k + 1))
+        s["ids"] = ((start + step * torch.arange(k, device="cuda")) % cols).to(torch.int32)
+        s["teacher"] = torch.sort(2 + 1.5 * normal(rows, k), dim=1, descending=True).values.contiguous()
+        count = torch.randint(0, 4 * k + 1, (rows,), generator=g, device="cuda").clamp_(max=k)
+        s["count"] = count.to(torch.int32)
+        s["temperature"] = 2.0
+        s["row_weight"] = (0.5 + torch.rand(rows, generator=g, device="cuda")) / rows
+        s["lse"] = torch.empty(rows, dtype=torch.float32, device="cuda")
+        if case["what"] == "grad":  # saved by the forward pass of the step
+            for r in range(0, rows, 256):
+                s["lse"][r:r + 256] = torch.logsumexp(logits[r:r + 256].double() / s["temperature"], 1).float()
+        s["loss"] = torch.empty(rows, dtype=torch.float32, device="cuda")
+        s["grad"] = _strided(rows, cols, pad, t) if case["what"] != "loss" else None
+        s["work"] = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
+    return s
+
+
+def _package():
+    if "trueno_rag_amd" in sys.modules:
+        return sys.modules["trueno_rag_amd"]
+    where = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "trueno-rag_amd")
+    spec = importlib.util.spec_from_file_location("trueno_rag_amd", os.path.join(where, "__init__.py"), submodule_search_locations=[where])
+    mod = importlib.util.module_from_spec(spec)
+    sys.modules["trueno_rag_amd"] = mod
+    spec.loader.exec_module(mod)
+    return mod
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _own_norm(s):
+    x, r = s["x"], s["residual_in"]
+    _package().rmsnorm_q8_device(x.data_ptr(), x.stride(0), _ptr(r), r.stride(0) if r is not None else 0, s["weight"].data_ptr(), _EPS,
+                                 _CODE[s["dtype"]], s["rows"], s["dim"], s["sum"].data_ptr() if r is not None else 0, s["sum"].stride(0),
+                                 s["q8"].data_ptr(), s["q8"].stride(0), s["scale"].data_ptr(), s["values"].data_ptr(), s["values"].stride(0),
+                                 torch.cuda.current_stream().cuda_stream)
+    return {"sum": s["sum"] if r is not None else None, "values": s["values"], "scale": s["scale"]}
+
+
+def _own_quantize(s):
+    x = s["x"]
+    _package().quantize_q8_device(x.data_ptr(), x.stride(0), _CODE[s["dtype"]], s["rows"], s["dim"], s["q8"].data_ptr(), s["q8"].stride(0),
+                                  s["scale"].data_ptr(), s["values"].data_ptr(), s["values"].stride(0), torch.cuda.current_stream().cuda_stream)
+    return {"values": s["values"], "scale": s["scale"]}
+
+
+def _own_product(s):
+    a, b, out = s["a"], s["b"], s["out"]
+    _package().matmul_q8_device(a.data_ptr(), a.stride(0), s["a_scale"].data_ptr(), b.data_ptr(), b.stride(0), s["b_scale"].data_ptr(),
+                                s["m"], s["n"], s["dim"], _CODE[s["to"]], out.data_ptr(), out.stride(0), torch.cuda.current_stream().cuda_stream)
+    return out
+
+
+def _own_distill(s):
+    p, z, grad = _package(), s["logits"], s["grad"]
+    lists = (s["ids"].data_ptr(), s["teacher"].data_ptr(), s["count"].data_ptr(), s["k"], s["temperature"])
+    if s["what"] == "grad":
+        p.distill_grad_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["lse"].data_ptr(),
+                              s["row_weight"].data_ptr(), grad.data_ptr(), grad.stride(0), torch.cuda.current_stream().cuda_stream)
+        return {"grad": grad}
+    step = s["what"] == "step"
+    p.distill_loss_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["loss"].data_ptr(), s["lse"].data_ptr(),
+                          s["row_weight"].data_ptr() if step else 0, _ptr(grad), grad.stride(0) if step else 0, s["work"].data_ptr(), s["work"].numel(),
+                          torch.cuda.current_stream().cuda_stream)
+    return {"loss": s["loss"], "lse": s["lse"], **({"grad": grad} if step else {})}
+
+
+def _plain_norm(s):
+    t = s["x"].dtype
+    # in single precision a step of the 8-bit grid is far more than the result's rounding: the quotient next to a border is taken in 64 bits
+    wide = torch.float64 if t == torch.float32 else torch.float32
+    x = s["x"].to(wide)
+    if s["residual_in"] is not None:
+        x = x + s["residual_in"].to(wide)
+    p = x * s["weight"].to(wide)
+    top = p.abs().amax(1, keepdim=True)
+    q = torch.round(p * 127 / top)
+    scale = top / 127 * torch.rsqrt((x * x).mean(1, keepdim=True) + _EPS)
+    return {"sum": x.to(t) if s["residual_in"] is not None else None, "values": (q * scale).to(t), "scale": scale.squeeze(1).float()}
+
+
+def _plain_quantize(s):
+    t = s["x"].dtype
+    x = s["x"].to(torch.float64 if t == torch.float32 else torch.float32)
+    top = x.abs().amax(1, keepdim=True)
+    scale = top / 127
+    return {"values": (torch.round(x * 127 / top) * scale).to(t), "scale": scale.squeeze(1).float()}
+
+
+def _plain_product(s):
+    c = s["a"].float() @ s["b"].float().t()
+    return (c * s["a_scale"][:, None] * s["b_scale"]).to(s["out"].dtype)
+
+
+def _teacher(s):
+    """The teacher's probabilities over its list: (rows, k), zero behind a list's end; all zero for an empty list."""
+    there = torch.arange(s["k"], device="cuda") < s["count"][:, None]
+    t = torch.where(there, s["teacher"] / s["temperature"], -torch.inf)
+    e = torch.where(there, torch.exp(t - t.amax(1, keepdim=True)), 0.0)
+    return e / e.sum(1, keepdim=True).clamp_min(1e-30), there
+
+
+def _plain_distill(s):
+    temp = s["temperature"]
+    z = s["logits"].float() / temp
+    p, there = _teacher(s)
+    some = (s["count"] > 0).float()
+    if s["what"] == "grad":
+        lse = s["lse"]
+    else:
+        top = z.amax(1, keepdim=True)
+        lse = (torch.log(torch.exp(z - top).sum(1, keepdim=True)) + top).squeeze(1)
+        at = torch.gather(z, 1, s["ids"].long())
+        loss = temp * temp * torch.where(p > 0, p * (torch.log(p) - at + lse[:, None]), 0.0).sum(1)
+        if s["what"] == "loss":
+            return {"loss": loss, "lse": lse}
+    d = torch.exp(z - lse[:, None]) * some[:, None]
+    d.scatter_add_(1, s["ids"].long(), -p)
+    d = (d * (temp * s["row_weight"])[:, None]).to(s["logits"].dtype)
+    return {"grad": d} if s["what"] == "grad" else {"loss": loss, "lse": lse, "grad": d}
+
+
+def run(s):
+    if own:
+        return {"norm": _own_norm, "quantize": _own_quantize, "product": _own_product, "distill": _own_distill}[s["op"]](s)
+    return {"norm": _plain_norm, "quantize": _plain_quantize, "product": _plain_product, "distill": _plain_distill}[s["op"]](s)
+
+
+def work(case):
+    op = case["op"]
+    if op in ("norm", "quantize"):
+        n, e = case["rows"] * case["dim"], _SIZE[case["dtype"]]
+        # the row in, (the other addend in, the sum out,) the integers and what they stand for out
+        per = e + 1 + e + (2 * e if op == "norm" and case["residual"] else 0)
+        return {"bytes": n * per + 4 * case["rows"] + (e * case["dim"] if op == "norm" else 0), "flops": 6 * n}
+    if op == "product":
+        m, n, dim = case["m"], case["n"], case["dim"]
+        return {"bytes": (m + n) * dim + 4 * (m + n) + m * n * _SIZE[case["to"]], "flops": 2 * m * n * dim}
+    n, e = case["rows"] * case["cols"], _SIZE[case["dtype"]]
+    return {"bytes": n * e * (1 if case["what"] == "loss" else 2) + case["rows"] * (8 * case["k"] + 16), "flops": 4 * n}
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "norm":
+        h = s["x"].double()
+        if case["residual"]:
+            h = h + s["residual_in"].double()
+        rms = (h.square().sum(1) / case["dim"] + _EPS).sqrt()
+        y = h * s["weight"].double()
+        step = y.abs().max(1).values / 127          # (before the norm: it cancels in the integers)
+        q = (y / step[:, None]).round()
+        return {"sum": h if case["residual"] else None, "values": q * (step / rms)[:, None], "scale": step / rms}
+    if case["op"] == "quantize":
+        x = s["x"].double()
+        step = x.abs().max(1).values / 127
+        return {"values": (x / step[:, None]).round() * step[:, None], "scale": step}
+    if case["op"] == "product":
+        a = s["a"].double() * s["a_scale"].double()[:, None]
+        return torch.cat([a @ (b.double() * w.double()[:, None]).t() for b, w in zip(s["b"].split(200_000), s["b_scale"].split(200_000))], 1)
+    temp, parts = s["temperature"], []
+    for r in range(0, case["rows"], 512):
+        z = s["logits"][r:r + 512].double() / temp
+        lse = z.logsumexp(1) if case["what"] != "grad" else s["lse"][r:r + 512].double()
+        logq = z - lse[:, None]
+        ids, n = s["ids"][r:r + 512].long(), s["count"][r:r + 512].long()
+        hidden = torch.arange(case["k"], device="cuda")[None] >= n[:, None]
+        t = (s["teacher"][r:r + 512].double() / temp).masked_fill(hidden, -torch.inf)
+        p = t.softmax(1).nan_to_num(0.0)
+        logp = t.log_softmax(1)
+        loss = temp ** 2 * (p * (logp - logq.gather(1, ids))).masked_fill(hidden, 0.0).sum(1)
+        grad = None
+        if case["what"] != "loss":
+            grad = (logq.exp().masked_fill((n == 0)[:, None], 0.0).scatter_add(1, ids, -p)
+                    * (temp * s["row_weight"][r:r + 512].double())[:, None])
+        parts.append((loss, lse, grad))
+    got = {"grad": torch.cat([g for _, _, g in parts])} if case["what"] != "loss" else {}
+    if case["what"] != "grad":
+        got.update(loss=torch.cat([x for x, _, _ in parts]), lse=torch.cat([x for _, x, _ in parts]))
+    return got
