@@ -141,10 +141,13 @@ def prepare(case, seed):
         s["count"] = count.to(torch.int32)
         s["temperature"] = 2.0
         s["row_weight"] = (0.5 + torch.rand(rows, generator=g, device="cuda")) / rows
-        s["lse"] = torch.empty(rows, dtype=torch.float32, device="cuda")
+        s["norm"] = torch.empty((rows, 2), dtype=torch.float32, device="cuda")  # a row's largest logit, log of its sum of exponentials
         if case["what"] == "grad":  # saved by the forward pass of the step
             for r in range(0, rows, 256):
-                s["lse"][r:r + 256] = torch.logsumexp(logits[r:r + 256].double() / s["temperature"], 1).float()
+                part = logits[r:r + 256].double()
+                top = part.amax(1)
+                s["norm"][r:r + 256, 0] = top.float()
+                s["norm"][r:r + 256, 1] = torch.logsumexp((part - top[:, None]) / s["temperature"], 1).float()
         s["loss"] = torch.empty(rows, dtype=torch.float32, device="cuda")
         s["grad"] = _strided(rows, cols, pad, t) if case["what"] != "loss" else None
         s["work"] = torch.empty(1 << 22, dtype=torch.uint8, device="cuda")
@@ -193,14 +196,14 @@ def _own_distill(s):
     p, z, grad = _package(), s["logits"], s["grad"]
     lists = (s["ids"].data_ptr(), s["teacher"].data_ptr(), s["count"].data_ptr(), s["k"], s["temperature"])
     if s["what"] == "grad":
-        p.distill_grad_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["lse"].data_ptr(),
+        p.distill_grad_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["norm"].data_ptr(),
                               s["row_weight"].data_ptr(), grad.data_ptr(), grad.stride(0), torch.cuda.current_stream().cuda_stream)
         return {"grad": grad}
     step = s["what"] == "step"
-    p.distill_loss_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["loss"].data_ptr(), s["lse"].data_ptr(),
+    p.distill_loss_device(z.data_ptr(), z.stride(0), _CODE[s["dtype"]], s["rows"], s["cols"], *lists, s["loss"].data_ptr(), s["norm"].data_ptr(),
                           s["row_weight"].data_ptr() if step else 0, _ptr(grad), grad.stride(0) if step else 0, s["work"].data_ptr(), s["work"].numel(),
                           torch.cuda.current_stream().cuda_stream)
-    return {"loss": s["loss"], "lse": s["lse"], **({"grad": grad} if step else {})}
+    return {"loss": s["loss"], "norm": s["norm"], **({"grad": grad} if step else {})}
 
 
 def _plain_norm(s):
@@ -235,27 +238,29 @@ def _teacher(s):
     there = torch.arange(s["k"], device="cuda") < s["count"][:, None]
     t = torch.where(there, s["teacher"] / s["temperature"], -torch.inf)
     e = torch.where(there, torch.exp(t - t.amax(1, keepdim=True)), 0.0)
-    return e / e.sum(1, keepdim=True).clamp_min(1e-30), there
+    return e / e.sum(1, keepdim=True).clamp_min(1e-30)
 
 
 def _plain_distill(s):
     temp = s["temperature"]
-    z = s["logits"].float() / temp
-    p, there = _teacher(s)
+    z = s["logits"].float()
+    p = _teacher(s)
     some = (s["count"] > 0).float()
+    top = s["norm"][:, :1] if s["what"] == "grad" else z.amax(1, keepdim=True)
+    z = (z - top) / temp
     if s["what"] == "grad":
-        lse = s["lse"]
+        log_sum = s["norm"][:, 1:]
     else:
-        top = z.amax(1, keepdim=True)
-        lse = (torch.log(torch.exp(z - top).sum(1, keepdim=True)) + top).squeeze(1)
+        log_sum = torch.log(torch.exp(z).sum(1, keepdim=True))
         at = torch.gather(z, 1, s["ids"].long())
-        loss = temp * temp * torch.where(p > 0, p * (torch.log(p) - at + lse[:, None]), 0.0).sum(1)
+        loss = temp * temp * torch.where(p > 0, p * (torch.log(p) - at + log_sum), 0.0).sum(1)
+        norm = torch.cat([top, log_sum], 1)
         if s["what"] == "loss":
-            return {"loss": loss, "lse": lse}
-    d = torch.exp(z - lse[:, None]) * some[:, None]
+            return {"loss": loss, "norm": norm}
+    d = torch.exp(z - log_sum) * some[:, None]
     d.scatter_add_(1, s["ids"].long(), -p)
     d = (d * (temp * s["row_weight"])[:, None]).to(s["logits"].dtype)
-    return {"grad": d} if s["what"] == "grad" else {"loss": loss, "lse": lse, "grad": d}
+    return {"grad": d} if s["what"] == "grad" else {"loss": loss, "norm": norm, "grad": d}
 
 
 def run(s):
@@ -298,9 +303,10 @@ def exact(case, seed):
         return torch.cat([a @ (b.double() * w.double()[:, None]).t() for b, w in zip(s["b"].split(200_000), s["b_scale"].split(200_000))], 1)
     temp, parts = s["temperature"], []
     for r in range(0, case["rows"], 512):
-        z = s["logits"][r:r + 512].double() / temp
-        lse = z.logsumexp(1) if case["what"] != "grad" else s["lse"][r:r + 512].double()
-        logq = z - lse[:, None]
+        z = s["logits"][r:r + 512].double()
+        top = z.max(1).values
+        log_sum = ((z - top[:, None]) / temp).logsumexp(1) if case["what"] != "grad" else s["norm"][r:r + 512, 1].double()
+        logq = (z - top[:, None]) / temp - log_sum[:, None]
         ids, n = s["ids"][r:r + 512].long(), s["count"][r:r + 512].long()
         hidden = torch.arange(case["k"], device="cuda")[None] >= n[:, None]
         t = (s["teacher"][r:r + 512].double() / temp).masked_fill(hidden, -torch.inf)
@@ -311,8 +317,8 @@ def exact(case, seed):
         if case["what"] != "loss":
             grad = (logq.exp().masked_fill((n == 0)[:, None], 0.0).scatter_add(1, ids, -p)
                     * (temp * s["row_weight"][r:r + 512].double())[:, None])
-        parts.append((loss, lse, grad))
+        parts.append((loss, torch.stack([top, log_sum], 1), grad))
     got = {"grad": torch.cat([g for _, _, g in parts])} if case["what"] != "loss" else {}
     if case["what"] != "grad":
-        got.update(loss=torch.cat([x for x, _, _ in parts]), lse=torch.cat([x for _, x, _ in parts]))
+        got.update(loss=torch.cat([x for x, _, _ in parts]), norm=torch.cat([x for _, x, _ in parts]))
     return got
