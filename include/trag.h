@@ -221,6 +221,13 @@ trag_status trag_store_fill_synthetic(trag_store *s, uint64_t n, uint64_t seed,
                                       uint64_t first_global_row, uint32_t *out_first_row);
 /* Copy rows [row0, row0+n) back to host memory (n x dim floats). */
 trag_status trag_store_read_rows(const trag_store *s, uint64_t row0, uint64_t n, float *out);
+/* Rows [row0, row0+n) as 8-bit integers with a scale each (trag_quantize_q8_device below, without leaving
+ * HBM): the corpus operand of trag_matmul_q8_device. d_q8 and d_scale are device arrays on the store's
+ * device; enqueued on hip_stream behind the handle's earlier work, as trag_store_search_device. Removed
+ * rows are written like the others. Row numbers out of range: TRAG_INVALID_ARG. Not for stream
+ * capture (TRAG_UNSUPPORTED): a replay would read rows that a growing store has moved. */
+trag_status trag_store_quantize_device(trag_store *s, uint64_t row0, uint32_t n, int8_t *d_q8,
+                                       uint64_t q8_stride, float *d_scale, void *hip_stream);
 
 /* FusionStrategy::fuse, src/fusion.rs:42-63. strategy: 0 RRF{k=param}
  * (:68-84), 1 Linear{dense_weight=param} (:87-109), 2 Convex{alpha=param}
@@ -493,6 +500,87 @@ trag_status trag_bm25_fill_synthetic(trag_bm25 *ix, uint64_t n_docs, uint32_t vo
 
 /* Diagnostics: postings held, distinct terms with at least one posting. */
 trag_status trag_bm25_stats(trag_bm25 *ix, uint64_t *postings, uint64_t *terms);
+
+/* ------------------------------------------------------------------------
+ * Operators on a caller's device arrays: an 8-bit first stage and the loss that trains its encoder.
+ * No counterpart in the reference (its embedder and its store are f32 throughout); the results they
+ * serve are those of VectorStore::search (src/index.rs:386-412). An encoder's hidden states become
+ * rows of 8-bit integers with one scale a row (trag_rmsnorm_q8_device), a corpus does so directly
+ * (trag_quantize_q8_device, trag_store_quantize_device), their product gives every score
+ * (trag_matmul_q8_device), and the lists of trag_store_search_device -- ids, scores and counts, as they
+ * are in device memory -- are the teacher of the loss (trag_distill_loss_device).
+ *
+ * All pointers are device pointers; work is enqueued on hip_stream and the call returns at once. The
+ * device is the stream's; with the default stream (NULL) it is the one the arrays live on, whatever
+ * the calling thread's current device. Arrays on another device, or in memory the device cannot read, are
+ * TRAG_INVALID_ARG. No call allocates, synchronises, or keeps anything: all may be captured into a
+ * graph and called by several threads. Strides count elements from row to row; rows may start at any
+ * element (16-byte alignment is not needed, and only the product goes faster with it). A call of 0
+ * rows is TRAG_OK and touches nothing. Outputs must not overlap inputs, except where said.
+ * ------------------------------------------------------------------------ */
+typedef enum trag_dtype { TRAG_F32 = 0, TRAG_F16 = 1, TRAG_BF16 = 2 } trag_dtype;
+
+/* Residual addition, root-mean-square norm and 8-bit rows in one pass. Per row of `dim` elements:
+ *   h = x + residual,   y = h * weight / sqrt(mean(h^2) + eps),
+ *   scale = max |y| / 127,   q8 = y / scale rounded to nearest, ties to even.
+ * h, y and the quotient are held in 64 bits: q8 is the same for any order of evaluation. d_residual
+ * NULL: none; d_weight NULL: ones. d_sum (may be NULL) receives h rounded to 32 bits and then to the
+ * rows' type; it may be d_x or d_residual itself, with that array's stride. d_values (may be NULL)
+ * receives q8 * scale in the rows' type, what the integers stand for; it may be d_x or d_residual
+ * likewise, but not d_sum. A row of zeros: scale 0 and integers 0. A row with an infinity or a NaN:
+ * scale NaN and integers 0, so that everything computed from it is NaN. dim <= 2^30. */
+trag_status trag_rmsnorm_q8_device(const void *d_x, uint64_t x_stride, const void *d_residual,
+                                   uint64_t residual_stride, const void *d_weight, float eps,
+                                   uint32_t dtype, uint32_t n_rows, uint32_t dim, void *d_sum,
+                                   uint64_t sum_stride, int8_t *d_q8, uint64_t q8_stride,
+                                   float *d_scale, void *d_values, uint64_t values_stride,
+                                   void *hip_stream);
+
+/* The same integers and scales of rows as they are: scale = max |x| / 127, q8 = x / scale. */
+trag_status trag_quantize_q8_device(const void *d_x, uint64_t x_stride, uint32_t dtype,
+                                    uint32_t n_rows, uint32_t dim, int8_t *d_q8, uint64_t q8_stride,
+                                    float *d_scale, void *d_values, uint64_t values_stride,
+                                    void *hip_stream);
+
+/* out[i][j] = (sum over k of a[i][k] * b[j][k]) * a_scale[i] * b_scale[j] for m rows of a (queries,
+ * tokens) and n rows of b (corpus rows, channels). A scale array may be NULL: ones. The integer sum is
+ * exact; it is rounded to f32, multiplied by a_scale[i] and then by b_scale[j] in f32, and rounded to
+ * the output's type. dim <= 131071 (the sum stays within 32 bits for every int8 value), and
+ * fewer than 2^24 tiles of 128 x 128 outputs, else TRAG_UNSUPPORTED. */
+trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const float *d_a_scale,
+                                  const int8_t *d_b, uint64_t b_stride, const float *d_b_scale,
+                                  uint32_t m, uint32_t n, uint32_t dim, uint32_t out_dtype,
+                                  void *d_out, uint64_t out_stride, void *hip_stream);
+
+/* Distillation from a teacher's best k. Row r of the teacher is the list of the first
+ * min(d_counts[r], k) pairs at r * k of d_ids (columns) and d_teacher (scores); d_counts NULL: all k. An
+ * id of n_cols or more marks an absent entry (it is left out, as if its score were minus infinity). The
+ * same id may stand in a list more than once; its probabilities add up. With T = temperature,
+ *   p = softmax(teacher / T) over the list,  q = softmax(logits / T) over the row,
+ *   loss[r] = T^2 * sum_j p_j (log p_j - log q[id_j]),
+ *   grad[r][c] = row_weight[r] * T * (q_c - sum of p_j with id_j = c).
+ * A row whose list is empty (or all minus infinity) is left out: loss 0 and gradient 0, whatever its
+ * logits. d_norm receives two floats a row, max(logits) and log sum exp((logits - max) / T): what
+ * trag_distill_grad_device needs. d_grad NULL: the loss alone; otherwise the gradient too, in the
+ * logits' type, for row weights known beforehand (d_row_weight, NULL: ones). d_grad may be d_logits
+ * itself, with its stride. d_work: trag_distill_work_bytes(n_rows, n_cols) bytes, 4-byte aligned, in use
+ * until the call's work is done (0 bytes, NULL, for rows of up to 32768 columns): two calls that can run at the same
+ * time, two captured graphs among them, need one each. k <= 1024, else TRAG_UNSUPPORTED. */
+uint64_t trag_distill_work_bytes(uint32_t n_rows, uint32_t n_cols);
+trag_status trag_distill_loss_device(const void *d_logits, uint64_t logits_stride, uint32_t dtype,
+                                     uint32_t n_rows, uint32_t n_cols, const uint32_t *d_ids,
+                                     const float *d_teacher, const uint32_t *d_counts, uint32_t k,
+                                     float temperature, float *d_loss, float *d_norm,
+                                     const float *d_row_weight, void *d_grad, uint64_t grad_stride,
+                                     void *d_work, uint64_t work_bytes, void *hip_stream);
+/* The gradient alone, from the d_norm of the forward call: for upstream gradients that exist only
+ * after it (d_row_weight = d total / d loss[r], NULL: ones). d_grad may be d_logits itself. */
+trag_status trag_distill_grad_device(const void *d_logits, uint64_t logits_stride, uint32_t dtype,
+                                     uint32_t n_rows, uint32_t n_cols, const uint32_t *d_ids,
+                                     const float *d_teacher, const uint32_t *d_counts, uint32_t k,
+                                     float temperature, const float *d_norm,
+                                     const float *d_row_weight, void *d_grad, uint64_t grad_stride,
+                                     void *hip_stream);
 
 /* `MockEmbedder::hash_to_vector` (src/embed.rs:124-155), the input generator
  * of the reference's tests and of benches/retrieval.rs: dim values from one

@@ -113,6 +113,7 @@ SIGNATURES = {
     "trag_store_has_bf16_mirror": (C.c_int, [_H]),
     "trag_store_scan_time": (C.c_int, [_H, C.POINTER(C.c_double), _u32p]),
     "trag_store_stream_probe": (C.c_int, [_H, C.c_uint32, C.POINTER(C.c_double)]),
+    "trag_store_quantize_device": (C.c_int, [_H, C.c_uint64, C.c_uint32, _H, C.c_uint64, _H, _H]),
     "trag_store_read_rows": (C.c_int, [_H, C.c_uint64, C.c_uint64, _fp]),
     "trag_fuse": (C.c_int, [C.c_uint32, C.c_float, _u64p, _fp, C.c_uint32, _u64p, _fp, C.c_uint32,
                             _u64p, _fp, _u32p]),
@@ -133,6 +134,17 @@ SIGNATURES = {
     "trag_bm25_fill_synthetic": (C.c_int, [_H, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64,
                                            _u32p]),
     "trag_bm25_stats": (C.c_int, [_H, _u64p, _u64p]),
+    "trag_rmsnorm_q8_device": (C.c_int, [_H, C.c_uint64, _H, C.c_uint64, _H, C.c_float, C.c_uint32, C.c_uint32, C.c_uint32,
+                                         _H, C.c_uint64, _H, C.c_uint64, _H, _H, C.c_uint64, _H]),
+    "trag_quantize_q8_device": (C.c_int, [_H, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, _H, C.c_uint64, _H, _H,
+                                          C.c_uint64, _H]),
+    "trag_matmul_q8_device": (C.c_int, [_H, C.c_uint64, _H, _H, C.c_uint64, _H, C.c_uint32, C.c_uint32, C.c_uint32,
+                                        C.c_uint32, _H, C.c_uint64, _H]),
+    "trag_distill_work_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32]),
+    "trag_distill_loss_device": (C.c_int, [_H, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, _H, _H, _H, C.c_uint32,
+                                           C.c_float, _H, _H, _H, _H, C.c_uint64, _H, C.c_uint64, _H]),
+    "trag_distill_grad_device": (C.c_int, [_H, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, _H, _H, _H, C.c_uint32,
+                                           C.c_float, _H, _H, _H, C.c_uint64, _H]),
     "trag_mock_embed": (C.c_int, [C.c_char_p, C.c_uint64, C.c_uint32, C.c_int, _fp]),
     "trag_last_error": (C.c_char_p, []),
     "trag_version": (C.c_char_p, []),

@@ -1490,6 +1490,27 @@ trag_status trag_store_read_rows(const trag_store* s, uint64_t row0, uint64_t n,
     return TRAG_OK;
 }
 
+trag_status trag_store_quantize_device(trag_store* s, uint64_t row0, uint32_t n, int8_t* d_q8, uint64_t q8_stride,
+                                       float* d_scale, void* hip_stream) {
+    if (!s) return fail(TRAG_INVALID_ARG, "null store");
+    std::lock_guard<std::mutex> lk(s->mu);
+    if (row0 + n > s->n_rows || row0 + n < row0) return fail(TRAG_INVALID_ARG, "row range out of bounds");
+    if (n == 0) return TRAG_OK;
+    if (!d_q8 || !d_scale) return fail(TRAG_INVALID_ARG, "null argument");
+    if (q8_stride < s->cfg.dim) return fail(TRAG_INVALID_ARG, "a row stride is less than the dimension");
+    DeviceGuard guard(s->device);
+    hipStream_t st = (hipStream_t)hip_stream;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if (st && hipStreamIsCapturing(st, &cap) != hipSuccess) { (void)hipGetLastError(); cap = hipStreamCaptureStatusNone; }
+    if (cap != hipStreamCaptureStatusNone)
+        return fail(TRAG_UNSUPPORTED, "a store's rows move when it grows: not for stream capture");
+    trag_status ts = order_after_last(s, st);   // (behind the copies of small inserts on the store's stream)
+    if (ts != TRAG_OK) return ts;
+    HIP_TRY(launch_quantize_rows_f32(s->d_rows + (size_t)row0 * s->cfg.dim, s->cfg.dim, n, s->cfg.dim, d_q8, q8_stride,
+                                     d_scale, st));
+    return TRAG_OK;
+}
+
 trag_status trag_store_search_device(trag_store* s, const float* d_queries, uint32_t n_queries,
                                      uint32_t dim, uint32_t k, uint32_t* d_out_rows,
                                      float* d_out_scores, uint32_t* d_out_n, uint32_t* d_status,

@@ -277,4 +277,8 @@ hipError_t launch_stream_probe(const float* d_rows, uint64_t n_floats, float* d_
 hipError_t launch_update_vmax(const float* d_rows, uint64_t n, uint32_t dim, float* d_vmax_sq,
                               float* d_norm2_out, hipStream_t st);
 
+// 8-bit rows with scales of f32 rows (trag_q8.hip)
+hipError_t launch_quantize_rows_f32(const float* d_rows, uint64_t stride, uint32_t n_rows, uint32_t dim, int8_t* d_q8,
+                                    uint64_t q8_stride, float* d_scale, hipStream_t st);
+
 }  // namespace trag

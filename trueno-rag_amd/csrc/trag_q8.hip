@@ -1,0 +1,312 @@
+// Rows of 8-bit integers with one scale a row: from an encoder's last step (residual addition and
+// root-mean-square norm) or from rows as they are (a corpus).
+//
+//   h = x + residual,  rms = sqrt(mean h^2 + eps),  y = h w / rms,
+//   scale = max |y| / 127,  q = nearest(y / scale), ties to even.
+//
+// The norm cancels in q: with p = h w it is nearest(127 p / max |p|), so the integers need one maximum
+// and the scale one sum, and both come out of ONE pass over the row, which stays in registers between
+// the loads and the stores. p, the maximum, the sum of squares and the quotient are held in 64 bits: a
+// quotient within a rounding of a border decides a whole step of the grid, and the 64-bit operations hide
+// behind the memory traffic that bounds the kernel. Without them q would depend on the order of f32
+// roundings; with them it is a function of the inputs alone.
+//
+// Bound by HBM: per element a read of x (and the residual), a write of the sum, of q and, if asked for, of
+// the values they stand for. One wave a row up to 1024 elements, one workgroup a row beyond; a row too
+// long for registers (over 32768 elements) is read twice, the second time from the caches.
+#include "trag_ops.h"
+
+namespace trag {
+namespace {
+
+struct Q8Args {
+    const void* x;
+    const void* residual;
+    const void* weight;
+    void* sum;
+    int8_t* q8;
+    float* scale;
+    void* values;
+    uint64_t x_stride, residual_stride, sum_stride, q8_stride, values_stride;
+    uint32_t n_rows, dim;
+    float eps;
+};
+
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+// nearest(127 p / top), ties to even. inv = 127 / top has its own rounding, which could move a tie off the
+// middle (or onto it): next to a border the side is taken from 127 p against the border times top.
+__device__ __forceinline__ int q8_nearest(double p, double inv, double top) {
+    const double t = p * inv;
+    double r = __builtin_rint(t);
+    if (__builtin_fabs(__builtin_fabs(t - r) - 0.5) < 1e-9) {
+        const double lo = __builtin_floor(t), c = lo + 0.5;
+        const double d = __builtin_fma(p, 127.0, -(c * top));
+        const double even = __builtin_rint(c);
+        r = d > 0.0 ? lo + 1.0 : (d < 0.0 ? lo : even);
+    }
+    return (int)r;
+}
+
+template <typename T, bool NORM>
+__device__ __forceinline__ void load_products(const Q8Args& a, const typename T::elem* x, const typename T::elem* res,
+                                              const typename T::elem* w, typename T::elem* sum, uint32_t e, bool write_sum,
+                                              double (&p)[8], double& ss) {
+    float xv[8], rv[8], wv[8];
+    const bool full = e + 8u <= a.dim;
+    if (full) {
+        T::load8(x + e, xv);
+        if (NORM && res) T::load8(res + e, rv);
+        if (NORM && w) T::load8(w + e, wv);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool in = e + (uint32_t)i < a.dim;
+            xv[i] = in ? T::load(x + e + i) : 0.0f;
+            if (NORM && res) rv[i] = in ? T::load(res + e + i) : 0.0f;
+            if (NORM && w) wv[i] = in ? T::load(w + e + i) : 0.0f;
+        }
+    }
+    if (NORM && sum && write_sum) {
+        float sv[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sv[i] = res ? xv[i] + rv[i] : xv[i];
+        if (full) T::store8(sum + e, sv);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (e + (uint32_t)i < a.dim) T::store(sum + e + i, sv[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        double h = (double)xv[i];
+        if (NORM && res) h += (double)rv[i];
+        p[i] = (NORM && w) ? h * (double)wv[i] : h;
+        if (NORM) ss = __builtin_fma(h, h, ss);
+        ss = __builtin_fma(p[i], 0.0, ss);   // (NaN as soon as a product is not finite; the maximum alone would pass over a NaN)
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row8(const Q8Args& a, int8_t* q8, typename T::elem* values, uint32_t e,
+                                           const double (&p)[8], double inv, double top, float scale) {
+    int q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = inv > 0.0 ? q8_nearest(p[i], inv, top) : 0;
+    if (e + 8u <= a.dim) {
+        u32x2_any o;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            o[h] = (uint32_t)(q[4 * h] & 255) | (uint32_t)(q[4 * h + 1] & 255) << 8 | (uint32_t)(q[4 * h + 2] & 255) << 16 |
+                   (uint32_t)q[4 * h + 3] << 24;
+        *reinterpret_cast<u32x2_any*>(q8 + e) = o;
+        if (values) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)q[i] * scale;
+            T::store8(values + e, v);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (e + (uint32_t)i < a.dim) {
+                q8[e + i] = (int8_t)q[i];
+                if (values) T::store(values + e + i, (float)q[i] * scale);
+            }
+    }
+}
+
+__device__ __forceinline__ double wave_max_f64(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = __builtin_fmax(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// From a row's maximum and sum: the factor of the integers (0: a row of zeros, or one that is not finite) and the scale.
+template <bool NORM>
+__device__ __forceinline__ void row_scale(const Q8Args& a, double top, double ss, double& inv, float& scale) {
+    const bool fine = ss - ss == 0.0;
+    inv = fine && top > 0.0 ? 127.0 / top : 0.0;
+    double s = top / 127.0;
+    if (NORM && top > 0.0) s /= __builtin_sqrt(ss / (double)a.dim + (double)a.eps);
+    scale = fine ? (float)s : __builtin_nanf("");
+}
+
+// NT threads a row (64: a wave a row, four rows a workgroup), NV vectors of eight elements a thread.
+// NV == 0: the row does not fit, it is read again for the integers.
+template <typename T, bool NORM, int NT, int NV>
+__global__ void __launch_bounds__(NT == 64 ? 256 : NT) q8_rows_kernel(const Q8Args a) {
+    typedef typename T::elem E;
+    constexpr int NW = NT / 64;
+    constexpr uint32_t RPB = NT == 64 ? 4u : 1u;
+    __shared__ double sh[2][NW > 1 ? NW : 1][2];
+    const uint32_t t = NT == 64 ? threadIdx.x & 63u : threadIdx.x;
+    const E* const w = reinterpret_cast<const E*>(a.weight);
+    uint32_t turn = 0;
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0u); row < a.n_rows;
+         row += (uint64_t)gridDim.x * RPB, turn ^= 1u) {
+        const E* const x = reinterpret_cast<const E*>(a.x) + row * a.x_stride;
+        const E* const res = a.residual ? reinterpret_cast<const E*>(a.residual) + row * a.residual_stride : nullptr;
+        E* const sum = a.sum ? reinterpret_cast<E*>(a.sum) + row * a.sum_stride : nullptr;
+        E* const values = a.values ? reinterpret_cast<E*>(a.values) + row * a.values_stride : nullptr;
+        int8_t* const q8 = a.q8 + row * a.q8_stride;
+        double top = 0.0, ss = 0.0;
+        double p[NV > 0 ? NV : 1][8];
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const uint32_t e = ((uint32_t)v * NT + t) * 8u;
+                if (e < a.dim) {
+                    load_products<T, NORM>(a, x, res, w, sum, e, true, p[v], ss);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = __builtin_fmax(top, __builtin_fabs(p[v][i]));
+                }
+            }
+        } else {
+            for (uint64_t e = t * 8u; e < a.dim; e += NT * 8u) {
+                load_products<T, NORM>(a, x, res, w, sum, (uint32_t)e, false, p[0], ss);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = __builtin_fmax(top, __builtin_fabs(p[0][i]));
+            }
+        }
+        top = wave_max_f64(top);
+        ss = wave_sum_f64(ss);
+        if constexpr (NW > 1) {
+            // (two turns of the array: a wave that is ahead writes the next row's partials beside the ones still read)
+            if ((threadIdx.x & 63u) == 0) { sh[turn][threadIdx.x >> 6][0] = top; sh[turn][threadIdx.x >> 6][1] = ss; }
+            __syncthreads();
+            top = sh[turn][0][0];
+            ss = sh[turn][0][1];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) { top = __builtin_fmax(top, sh[turn][i][0]); ss += sh[turn][i][1]; }
+        }
+        double inv;
+        float scale;
+        row_scale<NORM>(a, top, ss, inv, scale);
+        if (t == 0) a.scale[row] = scale;
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const uint32_t e = ((uint32_t)v * NT + t) * 8u;
+                if (e < a.dim) store_row8<T>(a, q8, values, e, p[v], inv, top, scale);
+            }
+        } else {
+            for (uint64_t e = t * 8u; e < a.dim; e += NT * 8u) {
+                double again = 0.0;
+                load_products<T, NORM>(a, x, res, w, sum, (uint32_t)e, true, p[0], again);
+                store_row8<T>(a, q8, values, (uint32_t)e, p[0], inv, top, scale);
+            }
+        }
+    }
+}
+
+template <typename T, bool NORM, int NT, int NV>
+void launch_one(const Q8Args& a, hipStream_t st) {
+    const uint32_t rpb = NT == 64 ? 4u : 1u;
+    const uint64_t blocks = ((uint64_t)a.n_rows + rpb - 1) / rpb;
+    const uint32_t grid = (uint32_t)(blocks < (1u << 20) ? blocks : (1u << 20));
+    hipLaunchKernelGGL((q8_rows_kernel<T, NORM, NT, NV>), dim3(grid), dim3(NT == 64 ? 256 : NT), 0, st, a);
+}
+
+template <typename T, bool NORM>
+void launch_type(const Q8Args& a, hipStream_t st) {
+    if (a.dim <= 512u) launch_one<T, NORM, 64, 1>(a, st);
+    else if (a.dim <= 1024u) launch_one<T, NORM, 64, 2>(a, st);
+    else if (a.dim <= 2048u) launch_one<T, NORM, 256, 1>(a, st);
+    else if (a.dim <= 4096u) launch_one<T, NORM, 256, 2>(a, st);
+    else if (a.dim <= 8192u) launch_one<T, NORM, 512, 2>(a, st);
+    else if (a.dim <= 16384u) launch_one<T, NORM, 1024, 2>(a, st);
+    else if (a.dim <= 32768u) launch_one<T, NORM, 1024, 4>(a, st);
+    else launch_one<T, NORM, 1024, 0>(a, st);
+}
+
+template <bool NORM>
+void launch_q8(const Q8Args& a, uint32_t dtype, hipStream_t st) {
+    if (dtype == TRAG_F32) launch_type<F32, NORM>(a, st);
+    else if (dtype == TRAG_F16) launch_type<F16, NORM>(a, st);
+    else launch_type<BF16, NORM>(a, st);
+}
+
+trag_status check_rows(const std::string& who, const Q8Args& a, uint32_t dtype) {
+    auto bad = [&](const char* what) { return set_error(TRAG_INVALID_ARG, who + ": " + what); };
+    if (dtype > TRAG_BF16) return bad("unknown element type");
+    if (a.dim == 0) return bad("dim is 0");
+    if (a.dim > (1u << 30)) return set_error(TRAG_UNSUPPORTED, who + ": dim is more than 2^30");
+    if (!a.x || !a.q8 || !a.scale) return bad("null array");
+    const uint32_t e = dtype_bytes(dtype);
+    if (!aligned_to(a.x, e) || !aligned_to(a.residual, e) || !aligned_to(a.weight, e) || !aligned_to(a.sum, e) ||
+        !aligned_to(a.values, e) || !aligned_to(a.scale, 4))
+        return bad("an array is not aligned to its elements");
+    if (a.x_stride < a.dim || (a.residual && a.residual_stride < a.dim) || (a.sum && a.sum_stride < a.dim) ||
+        a.q8_stride < a.dim || (a.values && a.values_stride < a.dim))
+        return bad("a row stride is less than dim");
+    // in place means the same rows: every thread reads what it later overwrites, nobody else does
+    if ((a.sum == a.x && a.sum && a.sum_stride != a.x_stride) || (a.sum && a.sum == a.residual && a.sum_stride != a.residual_stride) ||
+        (a.values && a.values == a.x && a.values_stride != a.x_stride) ||
+        (a.values && a.values == a.residual && a.values_stride != a.residual_stride))
+        return bad("an output in place of an input needs the input's stride");
+    if (a.values && a.values == a.sum) return bad("the sum and the values cannot share an array");
+    return TRAG_OK;
+}
+
+}  // namespace
+
+hipError_t launch_quantize_rows_f32(const float* d_rows, uint64_t stride, uint32_t n_rows, uint32_t dim, int8_t* d_q8,
+                                    uint64_t q8_stride, float* d_scale, hipStream_t st) {
+    Q8Args a{};
+    a.x = d_rows; a.x_stride = stride;
+    a.q8 = d_q8; a.q8_stride = q8_stride; a.scale = d_scale;
+    a.n_rows = n_rows; a.dim = dim;
+    launch_q8<false>(a, TRAG_F32, st);
+    return hipGetLastError();
+}
+
+}  // namespace trag
+
+extern "C" {
+
+trag_status trag_rmsnorm_q8_device(const void* d_x, uint64_t x_stride, const void* d_residual, uint64_t residual_stride,
+                                   const void* d_weight, float eps, uint32_t dtype, uint32_t n_rows, uint32_t dim,
+                                   void* d_sum, uint64_t sum_stride, int8_t* d_q8, uint64_t q8_stride, float* d_scale,
+                                   void* d_values, uint64_t values_stride, void* hip_stream) {
+    using namespace trag;
+    return op_entry([&]() -> trag_status {
+        const char* who = "trag_rmsnorm_q8_device";
+        if (n_rows == 0) return TRAG_OK;
+        const Q8Args a{d_x, d_residual, d_weight, d_sum, d_q8, d_scale, d_values, x_stride, residual_stride, sum_stride,
+                       q8_stride, values_stride, n_rows, dim, eps};
+        trag_status ts = check_rows(who, a, dtype);
+        if (ts != TRAG_OK) return ts;
+        if (!(eps >= 0.0f) || !(eps - eps == 0.0f)) return set_error(TRAG_INVALID_ARG, std::string(who) + ": eps must be finite and not negative");
+        OpDevice on(who, hip_stream, {d_x, d_residual, d_weight, d_sum, d_q8, d_scale, d_values});
+        if (on.status != TRAG_OK) return on.status;
+        launch_q8<true>(a, dtype, (hipStream_t)hip_stream);
+        return op_launched(who);
+    });
+}
+
+trag_status trag_quantize_q8_device(const void* d_x, uint64_t x_stride, uint32_t dtype, uint32_t n_rows, uint32_t dim,
+                                    int8_t* d_q8, uint64_t q8_stride, float* d_scale, void* d_values,
+                                    uint64_t values_stride, void* hip_stream) {
+    using namespace trag;
+    return op_entry([&]() -> trag_status {
+        const char* who = "trag_quantize_q8_device";
+        if (n_rows == 0) return TRAG_OK;
+        const Q8Args a{d_x, nullptr, nullptr, nullptr, d_q8, d_scale, d_values, x_stride, 0, 0, q8_stride, values_stride,
+                       n_rows, dim, 0.0f};
+        trag_status ts = check_rows(who, a, dtype);
+        if (ts != TRAG_OK) return ts;
+        OpDevice on(who, hip_stream, {d_x, d_q8, d_scale, d_values});
+        if (on.status != TRAG_OK) return on.status;
+        launch_q8<false>(a, dtype, (hipStream_t)hip_stream);
+        return op_launched(who);
+    });
+}
+
+}  // extern "C"
