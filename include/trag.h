@@ -546,7 +546,7 @@ trag_status trag_quantize_q8_device(const void *d_x, uint64_t x_stride, uint32_t
  * tokens) and n rows of b (corpus rows, channels). A scale array may be NULL: ones. The integer sum is
  * exact; it is rounded to f32, multiplied by a_scale[i] and then by b_scale[j] in f32, and rounded to
  * the output's type. dim <= 131071 (the sum stays within 32 bits for every int8 value), and
- * fewer than 2^24 tiles of 128 x 128 outputs, else TRAG_UNSUPPORTED. */
+ * fewer than 2^22 tiles of 128 x 128 outputs, else TRAG_UNSUPPORTED. */
 trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const float *d_a_scale,
                                   const int8_t *d_b, uint64_t b_stride, const float *d_b_scale,
                                   uint32_t m, uint32_t n, uint32_t dim, uint32_t out_dtype,
@@ -564,7 +564,7 @@ trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const fl
  * trag_distill_grad_device needs. d_grad NULL: the loss alone; otherwise the gradient too, in the
  * logits' type, for row weights known beforehand (d_row_weight, NULL: ones). d_grad may be d_logits
  * itself, with its stride. d_work: trag_distill_work_bytes(n_rows, n_cols) bytes, 4-byte aligned, in use
- * until the call's work is done (0 bytes, NULL, for rows of up to 32768 columns): two calls that can run at the same
+ * until the call's work is done (0 bytes, NULL, for rows of up to 65536 columns): two calls that can run at the same
  * time, two captured graphs among them, need one each. k <= 1024, else TRAG_UNSUPPORTED. */
 uint64_t trag_distill_work_bytes(uint32_t n_rows, uint32_t n_cols);
 trag_status trag_distill_loss_device(const void *d_logits, uint64_t logits_stride, uint32_t dtype,

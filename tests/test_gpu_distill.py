@@ -114,7 +114,7 @@ def _check_grad(got, want, tol, t):
     assert (off <= tol + eps * (want.abs() + tol) + TINY[t]).all(), (off.max().item(), (off - tol - eps * want.abs()).max().item())
 
 
-COLS = [1, 2, 7, 8, 9, 100, 1021, 2047, 2048, 2049, 4096, 4100, 8192, 8193, 16384, 16390, 32000, 32768, 32769, 40000, 70001, 152064]
+COLS = [1, 2, 7, 8, 9, 100, 1021, 2047, 2048, 2049, 4096, 4100, 8192, 8193, 16384, 16390, 32000, 32768, 32769, 40000, 65536, 65537, 70001, 152064]
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
@@ -179,7 +179,7 @@ def test_gradient_against_differences(trag):
         assert ((grad[:, c].double() - diff).abs() <= tol[:, c] + U * diff.abs() + 2 * temp * h * h + 1e-10).all()
 
 
-@pytest.mark.parametrize("cols", [300, 5000, 30000, 50000])
+@pytest.mark.parametrize("cols", [300, 1500, 5000, 30000, 50000, 90000])
 def test_masked_and_empty_rows(trag, cols):
     torch = _torch()
     inf, low = float("inf"), torch.finfo(torch.float32).min
@@ -221,7 +221,7 @@ def test_masked_and_empty_rows(trag, cols):
     assert torch.isnan(grad[0]).all() and torch.isnan(grad[1]).any()
 
 
-@pytest.mark.parametrize("cols", [64, 40000])
+@pytest.mark.parametrize("cols", [64, 40000, 80000])
 def test_empty_lists_of_length_zero_and_missing_counts(trag, cols):
     torch = _torch()
     z, ids, teacher, _, _ = _case(3, cols, 0, 1)
@@ -260,7 +260,7 @@ def test_a_row_past_32_bit_offsets(trag):
     _check_grad(z[449:], want[2], want[5] + want[1][:, 1:].abs() * 2 * U, "bf16")
 
 
-@pytest.mark.parametrize("cols", [3000, 60000])
+@pytest.mark.parametrize("cols", [3000, 60000, 120000])
 def test_streams_and_graphs(trag, cols):
     """A captured step replayed with new logits, two captured steps with a workspace each on two streams."""
     torch = _torch()

@@ -231,7 +231,8 @@ def _expect(a, b, sa, sb, dt):
 SHAPES = [(1, 1, 1), (1, 5, 16), (1, 1000, 384), (2, 129, 15), (3, 64, 17), (7, 300, 64), (8, 257, 768), (16, 4096, 1024),
           (17, 100, 63), (31, 513, 65), (32, 64, 128), (33, 4097, 96), (64, 640, 2048), (65, 130, 129), (100, 999, 250),
           (128, 128, 64), (129, 127, 144), (200, 2000, 384), (256, 256, 512), (257, 511, 400), (300, 1030, 777), (512, 768, 1040),
-          (1000, 300, 4096), (1025, 513, 48), (5, 3, 20000), (40, 70, 131071), (1, 40, 131071), (300, 300, 9000)]
+          (1000, 300, 4096), (1025, 513, 48), (5, 3, 20000), (300, 2000, 15), (2100, 2050, 1), (16, 4096, 4096), (33, 70, 4112),
+          (600, 4100, 2064), (1100, 4096, 1040), (2000, 9000, 272), (2050, 8200, 128), (70, 33000, 400), (40, 70, 131071), (1, 40, 131071), (300, 300, 9000)]
 
 
 @pytest.mark.parametrize("m,n,dim", SHAPES)
@@ -278,6 +279,22 @@ def test_product_past_32_bit_offsets(trag, m):
     _product(trag, a, b, None, None, out, "f32")
     for lo in (0, n // 2 - 500, n - 1000):
         assert torch.equal(out[:, lo:lo + 1000], _expect(a, b[lo:lo + 1000], None, None, torch.float32)), lo
+
+
+def test_product_of_rows_far_apart(trag):
+    """Strides of 2^24 bytes and more: offsets inside a tile pass 32 bits."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    far = (1 << 24) + 16
+    for m, n, dim in ((1, 300, 384), (70, 300, 100), (300, 40, 96)):
+        wide = torch.empty(300 * far + 512, dtype=torch.int8, device="cuda")
+        rows = torch.as_strided(wide, (300, dim), (far, 1))
+        rows.copy_(_int8(300, dim, 0, 0, g))
+        near = _int8(300, dim, 0, 0, g)
+        for a, b in ((near[:m], rows[:n]), (rows[:m], near[:n])):
+            out = torch.empty((m, n), device="cuda")
+            _product(trag, a, b, None, None, out, "f32")
+            assert torch.equal(out, _expect(a, b, None, None, torch.float32))
 
 
 def test_operators_on_other_streams_and_in_graphs(trag):

@@ -54,8 +54,8 @@ def test_product_refusals(trag, args, words):
 
 def test_product_limits(trag):
     _refused(trag, UNSUPPORTED, "131071", trag.matmul_q8_device, P, 131072, P, P, 131072, P, 4, 4, 131072, 0, P, 4)
-    big = 1 << 31
-    _refused(trag, UNSUPPORTED, "2^24 tiles", trag.matmul_q8_device, P, 64, P, P, 64, P, 200, big, 64, 0, P, big)
+    big = 1 << 29
+    _refused(trag, UNSUPPORTED, "2^22 tiles", trag.matmul_q8_device, P, 64, P, P, 64, P, 200, big, 64, 0, P, big)
     trag.matmul_q8_device(0, 0, 0, 0, 0, 0, 0, 4, 64, 0, 0, 0)
     trag.matmul_q8_device(0, 0, 0, 0, 0, 0, 4, 0, 64, 0, 0, 0)
 
@@ -72,8 +72,8 @@ def _loss(**kw):
     (dict(loss_ptr=0), "null"), (dict(norm_ptr=0), "null"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
     (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(logits_stride=99), "stride"),
     (dict(grad_stride=99), "stride"), (dict(grad_ptr=P, grad_stride=101), "in place"), (dict(logits_ptr=P + 2), "aligned"), (dict(ids_ptr=P + 2), "aligned"),
-    (dict(norm_ptr=P + 1), "aligned"), (dict(grad_ptr=P + 2), "aligned"), (dict(n_cols=40000, logits_stride=40000, grad_stride=40000), "workspace"),
-    (dict(n_cols=40000, logits_stride=40000, grad_stride=40000, work_ptr=P, work_bytes=8), "workspace")])
+    (dict(norm_ptr=P + 1), "aligned"), (dict(grad_ptr=P + 2), "aligned"), (dict(n_cols=80000, logits_stride=80000, grad_stride=80000), "workspace"),
+    (dict(n_cols=80000, logits_stride=80000, grad_stride=80000, work_ptr=P, work_bytes=8), "workspace")])
 def test_distill_refusals(trag, change, words):
     _refused(trag, INVALID, words, trag.distill_loss_device, **_loss(**change))
 
@@ -85,8 +85,8 @@ def test_distill_limits(trag):
     _refused(trag, INVALID, "null", trag.distill_grad_device, *a, 0, P, P, 100)
     _refused(trag, INVALID, "null", trag.distill_grad_device, *a, P, P, 0, 100)
     _refused(trag, INVALID, "stride", trag.distill_grad_device, *a, P, P, P + 4096, 99)
-    assert trag.distill_work_bytes(5, 32768) == 0 and trag.distill_work_bytes(0, 1 << 20) == 0
-    for rows, cols in ((1, 32769), (4096, 100_000), (64, 1_000_000), (1, (1 << 32) - 1), (1 << 20, 1 << 20)):
+    assert trag.distill_work_bytes(5, 65536) == 0 and trag.distill_work_bytes(0, 1 << 20) == 0
+    for rows, cols in ((1, 65537), (4096, 100_000), (64, 1_000_000), (1, (1 << 32) - 1), (1 << 20, 1 << 20)):
         need = trag.distill_work_bytes(rows, cols)
         assert need >= 8 * rows * -(-cols // 16384) and need % 8 == 0
 

@@ -19,8 +19,17 @@
 namespace trag {
 namespace {
 
+// f32 here goes by eight elements too, two 16-byte accesses a vector: half the branches of a row (4096 x 32000, loss and
+// gradient: 207 us, by four 239)
+struct F32by8 {
+    typedef float elem;
+    static constexpr int W = 8;
+    typedef float vec __attribute__((ext_vector_type(8), aligned(4)));
+    static __device__ __forceinline__ float round(float v) { return v; }
+};
+
 constexpr uint32_t LIST_MAX = 1024;        // teacher entries per row
-constexpr uint32_t ROW_MAX = 32768;        // columns of the row kernel
+constexpr uint32_t ROW_MAX = 65536;        // columns of the row kernel
 constexpr uint32_t PART_STEP = 2048;       // a chunk of a long row is a multiple of this
 constexpr uint32_t PART_MAX = 16384;
 
@@ -37,7 +46,9 @@ struct DistillArgs {
     float* parts;             // 2 per row and chunk
     uint64_t z_stride, grad_stride;
     uint32_t n_rows, n_cols, k, chunk, n_chunks;
+    uint32_t slot_mask;       // slots of the id table, a power of two, less one
     float temperature, c;     // c = log2(e) / T
+    double c64;
 };
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -45,186 +56,263 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 // exponent of e^((z - m) / T) as a power of two (off by three roundings, 3 * 2^-24 relative; an infinite z stays what it is)
 __device__ __forceinline__ float expo(const DistillArgs& a, float z, float m) { return (z - m) * a.c; }
 
-template <int NW>
-__device__ __forceinline__ float wg_max(float v, float* sh) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    if (NW == 1) return v;
-    if ((threadIdx.x & 63u) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) v = fmaxf(v, sh[i]);
     return v;
 }
-
-template <int NW>
-__device__ __forceinline__ double wg_sum(double v, double* sh) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    if (NW == 1) return v;
-    if ((threadIdx.x & 63u) == 0) sh[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) v += sh[i];
     return v;
 }
 
-// A row's teacher list, entry threadIdx.x + i * NT in slot i of each thread. An entry counts if it lies
-// in front of the row's count and its id is a column; p is 0 for the others. `some`: the list has
-// probability at all (an empty list, or one of minus infinities, leaves the row out: loss and gradient 0).
-template <int NT>
-struct TeacherList {
-    static constexpr int NL = (int)(LIST_MAX + NT - 1) / NT;
-    uint32_t id[NL];
-    float t[NL];
-    double p[NL], logp[NL];
-    bool there[NL];
-    bool some;
+// 2^x of a list's entry, to 3 * 2^-24: the whole part of x goes to the exponent, what is left is below one half
+__device__ __forceinline__ float list_exp(double x) {
+    if (x < -126.0) return 0.0f;
+    const double n = __builtin_rint(x);
+    return __builtin_ldexpf(exp2_hw((float)(x - n)), (int)n);
+}
 
-    __device__ __forceinline__ void load(const DistillArgs& a, uint64_t row) {
-        const uint32_t n = a.counts ? min(a.counts[row], a.k) : a.k;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const uint32_t j = threadIdx.x + (uint32_t)i * NT;
-            there[i] = j < n;
-            id[i] = there[i] ? a.ids[row * a.k + j] : 0u;
-            t[i] = there[i] ? a.teacher[row * a.k + j] : 0.0f;
-            there[i] = there[i] && id[i] < a.n_cols;
-        }
-    }
-    // sh_f, sh_d: NT / 64 words each, not shared with another reduction in between
-    __device__ __forceinline__ void softmax(const DistillArgs& a, float* sh_f, double* sh_d) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (there[i]) top = fmaxf(top, t[i]);   // (a NaN passes the maximum by and reaches the loss through its p)
-        top = wg_max<NT / 64>(top, sh_f);
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            // (a list of minus infinities: top is one, every difference would be NaN)
-            logp[i] = there[i] ? ((double)t[i] - (double)(top == -INFINITY ? 0.0f : top)) / (double)a.temperature : -INFINITY;
-            p[i] = there[i] ? exp(logp[i]) : 0.0;
-            sum += p[i];
-        }
-        sum = wg_sum<NT / 64>(sum, sh_d);
-        some = !(sum == 0.0);
-        const double ls = some ? log(sum) : 0.0;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            logp[i] -= ls;
-            p[i] = some ? p[i] / sum : 0.0;
-        }
-    }
+// Where a workgroup's waves meet: maxima of the row and of its teacher list, then three sums.
+template <int NW>
+struct Meet {
+    float top[2][NW];
+    double sum[3][NW];
 };
 
-// The gradient at the list's columns, after everything else of [c0, c1) has been written: the first entry of
-// an id takes the probabilities of all entries of that id. zl: the logits there, read before they may have been
-// overwritten (the gradient may go in place of the logits).
-template <typename T, int NT>
-__device__ __forceinline__ void patch_list(const DistillArgs& a, const TeacherList<NT>& l, const float (&zl)[TeacherList<NT>::NL],
-                                           typename T::elem* g, uint32_t c0, uint32_t c1, float m, float log2sum, float gt,
-                                           uint32_t* sh_id, float* sh_p) {
-#pragma unroll
-    for (int i = 0; i < TeacherList<NT>::NL; ++i) {
-        const uint32_t j = threadIdx.x + (uint32_t)i * NT;
-        if (j < a.k) { sh_id[j] = l.there[i] ? l.id[i] : 0xFFFFFFFFu; sh_p[j] = (float)l.p[i]; }
+// A row's teacher list in LDS, which is sized by the call: ids (NO_ID: an entry behind the row's count, or no column),
+// scores and later their exponentials, the logits at the ids. Entry j belongs to thread j % NT throughout. Behind it, for a
+// gradient, the first entry of every id and whether the id comes again: an open hash table of at least twice as many
+// slots as entries, filled anew for every row. Slots depend on who came first, what they say does not.
+struct List {
+    uint32_t* id;
+    float* e;
+    float* z;
+    uint32_t* slot_id;
+    uint32_t* slot_first;
+    uint32_t* slot_again;     // a bit a slot
+    __device__ __forceinline__ List(const DistillArgs& a, uint32_t* lds)
+        : id(lds), e(reinterpret_cast<float*>(lds + a.k)), z(reinterpret_cast<float*>(lds + 2u * a.k)), slot_id(lds + 3u * a.k),
+          slot_first(slot_id + a.slot_mask + 1u), slot_again(slot_first + a.slot_mask + 1u) {}
+};
+inline uint32_t list_bytes(const DistillArgs& a, bool table) {
+    return 4u * (3u * a.k + (table ? 2u * (a.slot_mask + 1u) + (a.slot_mask + 1u) / 32u : 0u));
+}
+constexpr uint32_t NO_ID = 0xFFFFFFFFu;   // (never a column: columns are below the number of columns)
+
+// p = softmax(t / T) over the list. `some`: the list has probability at all (an empty list, or one of minus
+// infinities, leaves the row out: loss and gradient 0).
+template <int NT>
+struct Teacher {
+    uint32_t id0;
+    float t0;
+    double sum;      // sum e, e = exp((t - max t) / T)
+    double cross;    // sum e ((t - max t) / T - (z_id - max z) / T)
+    bool some;
+
+    // Asked for ahead of the row: the first NT entries (whatever the row's count, so that the loads need not wait for it).
+    __device__ __forceinline__ void ask(const DistillArgs& a, uint64_t row) {
+        id0 = NO_ID;
+        t0 = 0.0f;
+        if (threadIdx.x < a.k) {
+            id0 = a.ids[row * a.k + threadIdx.x];
+            t0 = a.teacher[row * a.k + threadIdx.x];
+        }
+        const uint32_t n = a.counts ? min(a.counts[row], a.k) : a.k;
+        if (threadIdx.x >= n || id0 >= a.n_cols) id0 = NO_ID;
+        this->n = n;
     }
-    // what the workgroup has written so far is in memory, in front of what follows
-    __threadfence_block();
-    __syncthreads();
+    // The list into LDS, with the logits of the ids in [c0, c1); the largest score of this thread's entries.
+    template <typename T>
+    __device__ __forceinline__ float take(const DistillArgs& a, uint64_t row, const typename T::elem* z, uint32_t c0, uint32_t c1, const List& l) {
+        float top = -INFINITY;
+        uint32_t id = id0;
+        float t = t0;
+        for (uint32_t j = threadIdx.x; j < a.k; j += NT) {
+            if (j >= NT) {
+                id = a.ids[row * a.k + j];
+                t = a.teacher[row * a.k + j];
+                if (j >= n || id >= a.n_cols) id = NO_ID;
+            }
+            l.id[j] = id;
+            l.e[j] = t;
+            l.z[j] = id != NO_ID && id >= c0 && id < c1 ? (float)z[id] : 0.0f;
+            if (id != NO_ID) top = fmaxf(top, t);   // (a NaN passes the maximum by and reaches the loss through its exponential)
+        }
+        return top;
+    }
+    // this thread's part of the two sums; the exponentials replace the scores
+    __device__ __forceinline__ void sums(const DistillArgs& a, float top, float ref, const List& l) {
+        const float s0 = top == -INFINITY ? 0.0f : top;   // (a list of minus infinities: every difference would be NaN)
+        sum = cross = 0.0;
+        for (uint32_t j = threadIdx.x; j < a.k; j += NT) {
+            const float e = l.id[j] != NO_ID ? list_exp(((double)l.e[j] - (double)s0) * a.c64) : 0.0f;
+            sum += (double)e;
+            // (1 / T comes with the sum: write_row)
+            if (!(e == 0.0f)) cross += (double)e * (((double)l.e[j] - (double)s0) - ((double)l.z[j] - (double)ref));
+            l.e[j] = e;
+        }
+    }
+    static __device__ __forceinline__ void clear(const DistillArgs& a, const List& l) {
+        for (uint32_t s = threadIdx.x; s <= a.slot_mask; s += NT) {
+            l.slot_id[s] = NO_ID;
+            l.slot_first[s] = NO_ID;
+            if ((s & 31u) == 0u) l.slot_again[s >> 5] = 0u;
+        }
+    }
+    static __device__ __forceinline__ uint32_t home(const DistillArgs& a, uint32_t id) { return (id * 2654435761u) >> 21 & a.slot_mask; }
+    // (a barrier after clear, and one before patch)
+    static __device__ __forceinline__ void enter(const DistillArgs& a, const List& l, uint32_t c0, uint32_t c1) {
+        for (uint32_t j = threadIdx.x; j < a.k; j += NT) {
+            const uint32_t id = l.id[j];
+            if (id == NO_ID || id < c0 || id >= c1) continue;
+            uint32_t s = home(a, id), was;
+            while ((was = atomicCAS(&l.slot_id[s], NO_ID, id)) != NO_ID && was != id) s = (s + 1u) & a.slot_mask;   // (half of the slots are free)
+            if (was == id) atomicOr(&l.slot_again[s >> 5], 1u << (s & 31u));
+            atomicMin(&l.slot_first[s], j);
+        }
+    }
+    // (after the sums of all threads are in)
+    __device__ __forceinline__ void finish() { some = !(sum == 0.0); }
+    // The gradient at the list's columns, after everything else of [c0, c1) has been written: the first entry of an id
+    // takes the probabilities of all entries of that id, in the list's order. (The logits there come from the list: the
+    // gradient may have gone in their place.)
+    template <typename T>
+    __device__ __forceinline__ void patch(const DistillArgs& a, const List& l, typename T::elem* g, uint32_t c0, uint32_t c1,
+                                          float ref, float per_sum, float gt) const {
+        const float inv = (float)(1.0 / sum);
+        for (uint32_t j = threadIdx.x; j < a.k; j += NT) {
+            const uint32_t id = l.id[j];
+            if (id == NO_ID || id < c0 || id >= c1) continue;
+            uint32_t s = home(a, id);
+            while (l.slot_id[s] != id) s = (s + 1u) & a.slot_mask;   // (it has been entered)
+            if (l.slot_first[s] != j) continue;
+            float e = l.e[j];
+            if (l.slot_again[s >> 5] >> (s & 31u) & 1u)
+#pragma unroll 8
+                for (uint32_t o = j + 1u; o < a.k; ++o) e += l.id[o] == id ? l.e[o] : 0.0f;
+            g[id] = T::round(gt * (exp2_hw(expo(a, l.z[j], ref)) * per_sum - e * inv));
+        }
+    }
+
+  private:
+    uint32_t n;
+};
+
+// what a row's sums come to: loss = T^2 (sum p (log p - log q)) = T^2 (cross / sum / T - log sum + log of the row's sum)
+template <int NT>
+__device__ __forceinline__ void write_row(const DistillArgs& a, uint64_t row, float m, double row_sum, const Teacher<NT>& l) {
+    const double ln = log(row_sum), temp = (double)a.temperature;
+    a.loss[row] = l.some ? (float)(temp * (l.cross / l.sum) + temp * temp * (ln - log(l.sum))) : 0.0f;
+    a.norm[2 * row] = m;
+    a.norm[2 * row + 1] = (float)ln;
+}
+
+// 16-bit types: what is carried on is the row as it is in memory; without this the compiler keeps the converted floats
+// from one pass to the next, in twice the registers
+template <typename T, int NV>
+__device__ __forceinline__ void keep_raw(typename T::vec (&h)[NV]) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    if constexpr (sizeof(typename T::elem) == 2) {
 #pragma unroll
-    for (int i = 0; i < TeacherList<NT>::NL; ++i) {
-        const uint32_t j = threadIdx.x + (uint32_t)i * NT;
-        if (j >= a.k || !l.there[i] || l.id[i] < c0 || l.id[i] >= c1) continue;
-        bool first = true;
-        for (uint32_t o = 0; o < j; ++o) first = first && sh_id[o] != l.id[i];
-        if (!first) continue;
-        float p = 0.0f;
-        for (uint32_t o = j; o < a.k; ++o)
-            if (sh_id[o] == l.id[i]) p += sh_p[o];
-        const float q = exp2_hw(expo(a, zl[i], m) - log2sum);
-        T::store(g + l.id[i], gt * (q - p));
+        for (int v = 0; v < NV; ++v) {
+            u32x4 w = __builtin_bit_cast(u32x4, h[v]);
+            asm volatile("" : "+v"(w));
+            h[v] = __builtin_bit_cast(typename T::vec, w);
+        }
     }
 }
 
-// One workgroup a row, the row in registers: NV vectors of eight columns a thread.
+// One workgroup a row, the row in registers as NV vectors of W columns a thread (the columns behind the last
+// whole vector: one each for the first few threads): one read of the logits, one write of the gradient, two meetings
+// of the waves and one more before the list's columns are set right.
 template <typename T, int NT, int NV, bool GRAD>
-__global__ void __launch_bounds__(NT) distill_row_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(NT, NT == 256 && sizeof(typename T::elem) == 2 && NV == 16 ? 3 : 1) distill_row_kernel(const DistillArgs a) {
     typedef typename T::elem E;
-    constexpr int NW = NT / 64, NL = TeacherList<NT>::NL;
-    __shared__ float sh_f[2][NW];
-    __shared__ double sh_d[3][NW];
-    __shared__ uint32_t sh_id[GRAD ? LIST_MAX : 1];
-    __shared__ float sh_p[GRAD ? LIST_MAX : 1];
+    constexpr int NW = NT / 64;
+    __shared__ Meet<NW> meet;
+    extern __shared__ uint32_t lds[];
+    const List list(a, lds);
+    const uint32_t wid = threadIdx.x >> 6;
+    const bool lead = (threadIdx.x & 63u) == 0u;
+    const uint32_t whole = a.n_cols / T::W * T::W, ct = whole + threadIdx.x;
     for (uint64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
         const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-        float e[NV][8];
-        float m = -INFINITY;
+        Teacher<NT> l;
+        l.ask(a, row);
+        // (held as they are in memory; in f32 the exponentials take their place, 16-bit types compute them again for the
+        // gradient, which costs less than the occupancy that twice the registers would)
+        // (Loads clamped to the row's last vector instead of the branches, the excess masked: 53.8 us instead of 48.6 for the
+        // loss of 4096 x 32000 bf16, no faster with the gradient.)
+        typename T::vec h[NV];
+        float et = -INFINITY;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * 8u;
-            if (c + 8u <= a.n_cols) T::load8(z + c, e[v]);
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) e[v][i] = c + (uint32_t)i < a.n_cols ? T::load(z + c + i) : -INFINITY;
-            }
+            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+            h[v] = fill_vec<T>(-INFINITY);
+            if (c < whole) h[v] = load_vec<T>(z + c);
         }
-        TeacherList<NT> l;
-        l.load(a, row);
-        float zl[NL];
-#pragma unroll
-        for (int i = 0; i < NL; ++i) zl[i] = l.there[i] ? T::load(z + l.id[i]) : 0.0f;
+        if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) et = (float)z[ct];
+        if constexpr (GRAD) l.clear(a, list);
+        float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
+        float m = et;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, e[v][i]);
-        m = wg_max<NW>(m, sh_f[0]);
+            for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
+        keep_raw<T, NV>(h);
+        m = wave_max(m);
+        if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
         const float ref = m == -INFINITY ? 0.0f : m;
-        float s = 0.0f;
+        if constexpr (GRAD) l.enter(a, list, 0u, a.n_cols);
+        l.sums(a, lt, ref, list);
+        et = exp2_hw(expo(a, et, ref));
+        float s = et;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                e[v][i] = exp2_hw(expo(a, e[v][i], ref));
-                s += e[v][i];
+            for (int i = 0; i < T::W; ++i) {
+                const float x = exp2_hw(expo(a, (float)h[v][i], ref));
+                s += x;
+                if constexpr (GRAD && sizeof(E) == 4) h[v][i] = x;
             }
-        const double sum = wg_sum<NW>((double)s, sh_d[0]);
-        l.softmax(a, sh_f[1], sh_d[1]);
-        const double ln = log(sum);
-        double part = 0.0;
+        if constexpr (GRAD) keep_raw<T, NV>(h);
+        double sum = wave_sum((double)s);
+        l.sum = wave_sum(l.sum);
+        l.cross = wave_sum(l.cross);
+        if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
+        __syncthreads();
+        sum = l.sum = l.cross = 0.0;
 #pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (l.there[i] && !(l.p[i] == 0.0))
-                part += l.p[i] * (l.logp[i] - ((double)zl[i] - (double)ref) / (double)a.temperature + ln);
-        part = wg_sum<NW>(part, sh_d[2]);
-        if (threadIdx.x == 0) {
-            a.loss[row] = l.some ? (float)((double)a.temperature * (double)a.temperature * part) : 0.0f;
-            a.norm[2 * row] = m;
-            a.norm[2 * row + 1] = (float)ln;
-        }
+        for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
+        l.finish();
         if constexpr (GRAD) {
             E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
             const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
             const float f = (float)((double)gt / sum);
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * 8u;
-                float o[8];
+                const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+                typename T::vec o;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] = l.some ? e[v][i] * f : 0.0f;
-                if (c + 8u <= a.n_cols) T::store8(g + c, o);
-                else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (c + (uint32_t)i < a.n_cols) T::store(g + c + i, o[i]);
+                for (int i = 0; i < T::W; ++i) {
+                    const float x = sizeof(E) == 4 ? (float)h[v][i] : exp2_hw(expo(a, (float)h[v][i], ref));
+                    o[i] = T::round(l.some ? x * f : 0.0f);
                 }
+                if (c < whole) store_vec<T>(g + c, o);
             }
-            if (l.some) patch_list<T, NT>(a, l, zl, g, 0, a.n_cols, ref, (float)(ln * 1.4426950408889634), gt, sh_id, sh_p);
+            if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) g[ct] = T::round(l.some ? et * f : 0.0f);
+            // what the workgroup has written so far is in memory, in front of what follows
+            __threadfence_block();
+            __syncthreads();
+            if (l.some) l.template patch<T>(a, list, g, 0u, a.n_cols, ref, (float)(1.0 / sum), gt);
         }
-        __syncthreads();   // the next row's reductions and lists reuse the arrays
+        if (threadIdx.x == 0) write_row(a, row, m, sum, l);
+        __syncthreads();   // (the next row uses the same arrays)
     }
 }
 
@@ -233,37 +321,47 @@ template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     typedef typename T::elem E;
     constexpr int NW = NT / 64;
-    __shared__ float sh_f[NW];
-    __shared__ double sh_d[NW];
+    __shared__ Meet<NW> meet;
+    const uint32_t wid = threadIdx.x >> 6;
+    const bool lead = (threadIdx.x & 63u) == 0u;
     const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
     for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
         const uint64_t row = part / a.n_chunks;
         const uint64_t c0 = (part % a.n_chunks) * a.chunk, c1 = min(c0 + a.chunk, (uint64_t)a.n_cols);
         const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
         float m = -INFINITY, s = 0.0f;
-        for (uint64_t c = c0 + threadIdx.x * 8u; c < c1; c += NT * 8u) {
-            float e[8];
-            if (c + 8u <= c1) T::load8(z + c, e);
-            else {
+        const uint64_t ct = c0 + (c1 - c0) / T::W * T::W + threadIdx.x;   // (the columns behind the last whole vector, one each)
+        if (threadIdx.x < (uint32_t)T::W && ct < c1) {
+            m = (float)z[ct];
+            s = m == m ? (m == -INFINITY ? 0.0f : (m - m == 0.0f ? 1.0f : m - m)) : m;
+            if (m != m) m = -INFINITY;
+        }
+        for (uint64_t c = c0 + threadIdx.x * T::W; c + T::W <= c1; c += NT * T::W) {
+            const typename T::vec e = load_vec<T>(z + c);
+            float top = (float)e[0];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = c + (uint32_t)i < c1 ? T::load(z + c + i) : -INFINITY;
-            }
-            float top = e[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) top = fmaxf(top, e[i]);
+            for (int i = 1; i < T::W; ++i) top = fmaxf(top, (float)e[i]);
             if (top > m) {   // (rare after the first few: the maximum of a random sequence moves ln n times)
                 s = m == -INFINITY ? s : s * exp2_hw(expo(a, m, top));
                 m = top;
             }
             const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += exp2_hw(expo(a, e[i], ref));
+            for (int i = 0; i < T::W; ++i) s += exp2_hw(expo(a, (float)e[i], ref));
         }
-        const float top = wg_max<NW>(m, sh_f);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        const float f = m == -INFINITY ? 1.0f : exp2_hw(expo(a, m, ref));
-        const double sum = wg_sum<NW>((double)s * (double)f, sh_d);
+        // (each wave's sum at its own maximum, then both to the workgroup's)
+        const float wm = wave_max(m), wref = wm == -INFINITY ? 0.0f : wm;
+        const double ws = wave_sum((double)s * (double)(m == -INFINITY ? 1.0f : exp2_hw(expo(a, m, wref))));
+        if (lead) { meet.top[0][wid] = wm; meet.sum[0][wid] = ws; }
+        __syncthreads();
         if (threadIdx.x == 0) {
+            float top = meet.top[0][0];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, meet.top[0][w]);
+            double sum = 0.0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+                sum += meet.sum[0][w] * (meet.top[0][w] == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, meet.top[0][w], top)));
             a.parts[2 * part] = top;
             a.parts[2 * part + 1] = (float)sum;
         }
@@ -275,41 +373,44 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
     typedef typename T::elem E;
-    constexpr int NW = NT / 64, NL = TeacherList<NT>::NL;
-    __shared__ float sh_f[2][NW];
-    __shared__ double sh_d[3][NW];
+    constexpr int NW = NT / 64;
+    __shared__ Meet<NW> meet;
+    extern __shared__ uint32_t lds[];
+    const List list(a, lds);
+    const uint32_t wid = threadIdx.x >> 6;
+    const bool lead = (threadIdx.x & 63u) == 0u;
     for (uint64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
         const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
         const float* const parts = a.parts + 2 * row * a.n_chunks;
-        TeacherList<NT> l;
-        l.load(a, row);
-        float zl[NL];
-#pragma unroll
-        for (int i = 0; i < NL; ++i) zl[i] = l.there[i] ? T::load(z + l.id[i]) : 0.0f;
+        Teacher<NT> l;
+        l.ask(a, row);
+        float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
+        // (a thread's chunks at the thread's own maximum, then to the row's)
         float m = -INFINITY;
         for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) m = fmaxf(m, parts[2 * c]);
-        m = wg_max<NW>(m, sh_f[0]);
+        m = wave_max(m);
+        if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
         const float ref = m == -INFINITY ? 0.0f : m;
-        double s = 0.0;
+        double sum = 0.0;
         for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) {
             const float pm = parts[2 * c];
             // (a chunk without a number: its sum is 0, or NaN, and stays that)
-            s += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
+            sum += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
         }
-        const double sum = wg_sum<NW>(s, sh_d[0]);
-        l.softmax(a, sh_f[1], sh_d[1]);
-        const double ln = log(sum);
-        double part = 0.0;
+        l.sums(a, lt, ref, list);
+        sum = wave_sum(sum);
+        l.sum = wave_sum(l.sum);
+        l.cross = wave_sum(l.cross);
+        if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
+        __syncthreads();
+        sum = l.sum = l.cross = 0.0;
 #pragma unroll
-        for (int i = 0; i < NL; ++i)
-            if (l.there[i] && !(l.p[i] == 0.0))
-                part += l.p[i] * (l.logp[i] - ((double)zl[i] - (double)ref) / (double)a.temperature + ln);
-        part = wg_sum<NW>(part, sh_d[2]);
-        if (threadIdx.x == 0) {
-            a.loss[row] = l.some ? (float)((double)a.temperature * (double)a.temperature * part) : 0.0f;
-            a.norm[2 * row] = m;
-            a.norm[2 * row + 1] = (float)ln;
-        }
+        for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
+        l.finish();
+        if (threadIdx.x == 0) write_row(a, row, m, sum, l);
         __syncthreads();
     }
 }
@@ -318,45 +419,52 @@ __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     typedef typename T::elem E;
-    constexpr int NW = NT / 64, NL = TeacherList<NT>::NL;
-    __shared__ float sh_f[NW];
-    __shared__ double sh_d[NW];
-    __shared__ uint32_t sh_id[LIST_MAX];
-    __shared__ float sh_p[LIST_MAX];
+    constexpr int NW = NT / 64;
+    __shared__ Meet<NW> meet;
+    extern __shared__ uint32_t lds[];
+    const List list(a, lds);
+    const uint32_t wid = threadIdx.x >> 6;
+    const bool lead = (threadIdx.x & 63u) == 0u;
     const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
     for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
         const uint64_t row = part / a.n_chunks;
         const uint64_t c0 = (part % a.n_chunks) * a.chunk, c1 = min(c0 + a.chunk, (uint64_t)a.n_cols);
         const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
         E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
-        TeacherList<NT> l;
-        l.load(a, row);
-        float zl[NL];
+        Teacher<NT> l;
+        l.ask(a, row);
+        l.clear(a, list);
+        float lt = wave_max(l.template take<T>(a, row, z, (uint32_t)c0, (uint32_t)c1, list));
+        if (lead) meet.top[1][wid] = lt;
+        __syncthreads();   // (the logits of the list have been read before any is overwritten)
 #pragma unroll
-        for (int i = 0; i < NL; ++i) zl[i] = l.there[i] && l.id[i] >= c0 && l.id[i] < c1 ? T::load(z + l.id[i]) : 0.0f;
-        l.softmax(a, sh_f, sh_d);   // (its barriers also stand between the reads of zl and the writes below)
+        for (int w = 0; w < NW; ++w) lt = fmaxf(lt, meet.top[1][w]);
+        l.enter(a, list, (uint32_t)c0, (uint32_t)c1);
+        l.sums(a, lt, 0.0f, list);
+        l.sum = wave_sum(l.sum);
+        if (lead) meet.sum[1][wid] = l.sum;
+        __syncthreads();
+        l.sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) l.sum += meet.sum[1][w];
+        l.finish();
         const float m = a.norm_in[2 * row];
         const float ref = m == -INFINITY ? 0.0f : m;
-        const float log2sum = (float)((double)a.norm_in[2 * row + 1] * 1.4426950408889634);
+        const float per_sum = (float)exp(-(double)a.norm_in[2 * row + 1]);
         const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
-        for (uint64_t c = c0 + threadIdx.x * 8u; c < c1; c += NT * 8u) {
-            float e[8];
-            const bool full = c + 8u <= c1;
-            if (full) T::load8(z + c, e);
-            else {
+        const float f = gt * per_sum;
+        const uint64_t ct = c0 + (c1 - c0) / T::W * T::W + threadIdx.x;
+        if (threadIdx.x < (uint32_t)T::W && ct < c1) g[ct] = T::round(l.some ? f * exp2_hw(expo(a, (float)z[ct], ref)) : 0.0f);
+        for (uint64_t c = c0 + threadIdx.x * T::W; c + T::W <= c1; c += NT * T::W) {
+            const typename T::vec e = load_vec<T>(z + c);
+            typename T::vec o;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = c + (uint32_t)i < c1 ? T::load(z + c + i) : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = l.some ? gt * exp2_hw(expo(a, e[i], ref) - log2sum) : 0.0f;
-            if (full) T::store8(g + c, e);
-            else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (c + (uint32_t)i < c1) T::store(g + c + i, e[i]);
-            }
+            for (int i = 0; i < T::W; ++i) o[i] = T::round(l.some ? f * exp2_hw(expo(a, (float)e[i], ref)) : 0.0f);
+            store_vec<T>(g + c, o);
         }
-        if (l.some) patch_list<T, NT>(a, l, zl, g, (uint32_t)c0, (uint32_t)c1, ref, log2sum, gt, sh_id, sh_p);
+        __threadfence_block();
+        __syncthreads();
+        if (l.some) l.template patch<T>(a, list, g, (uint32_t)c0, (uint32_t)c1, ref, per_sum, gt);
         __syncthreads();
     }
 }
@@ -377,27 +485,30 @@ void set_chunks(DistillArgs& a) {
 
 template <typename T, int NT, int NV>
 void launch_row(const DistillArgs& a, hipStream_t st) {
-    if (a.grad) hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, true>), dim3(grid_of(a.n_rows)), dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, false>), dim3(grid_of(a.n_rows)), dim3(NT), 0, st, a);
+    if (a.grad) hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, true>), dim3(grid_of(a.n_rows)), dim3(NT), list_bytes(a, true), st, a);
+    else hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, false>), dim3(grid_of(a.n_rows)), dim3(NT), list_bytes(a, false), st, a);
 }
 
 template <typename T>
 void launch_grad(const DistillArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((distill_grad_kernel<T, 256>), dim3(grid_of((uint64_t)a.n_rows * a.n_chunks)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((distill_grad_kernel<T, 256>), dim3(grid_of((uint64_t)a.n_rows * a.n_chunks)), dim3(256), list_bytes(a, true), st, a);
 }
 
 template <typename T>
 void launch_loss(DistillArgs a, hipStream_t st) {
     if (a.n_cols <= ROW_MAX) {
-        if (a.n_cols <= 2048u) launch_row<T, 256, 1>(a, st);
+        if (a.n_cols <= 512u) launch_row<T, 64, 1>(a, st);
+        else if (a.n_cols <= 1024u) launch_row<T, 64, 2>(a, st);
+        else if (a.n_cols <= 2048u) launch_row<T, 128, 2>(a, st);
         else if (a.n_cols <= 4096u) launch_row<T, 256, 2>(a, st);
         else if (a.n_cols <= 8192u) launch_row<T, 256, 4>(a, st);
-        else if (a.n_cols <= 16384u) launch_row<T, 512, 4>(a, st);
-        else launch_row<T, 1024, 4>(a, st);
+        else if (a.n_cols <= 16384u) launch_row<T, 256, 8>(a, st);
+        else if (a.n_cols <= 32768u) launch_row<T, 256, 16>(a, st);
+        else launch_row<T, 512, 16>(a, st);
         return;
     }
     hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(grid_of((uint64_t)a.n_rows * a.n_chunks)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3(grid_of(a.n_rows)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3(grid_of(a.n_rows)), dim3(256), list_bytes(a, false), st, a);
     if (a.grad) {
         a.norm_in = a.norm;
         launch_grad<T>(a, st);
@@ -432,8 +543,12 @@ DistillArgs distill_args(const void* z, uint64_t z_stride, uint32_t n_rows, uint
     DistillArgs a{};
     a.z = z; a.z_stride = z_stride; a.n_rows = n_rows; a.n_cols = n_cols;
     a.ids = ids; a.teacher = teacher; a.counts = counts; a.k = k; a.temperature = temperature;
-    a.c = (float)(1.4426950408889634 / (double)temperature);
+    a.c64 = 1.4426950408889634 / (double)temperature;
+    a.c = (float)a.c64;
     if (n_rows && n_cols) set_chunks(a);
+    uint32_t slots = 64;
+    while (slots < 2u * k && slots < 2u * LIST_MAX) slots *= 2u;
+    a.slot_mask = slots - 1u;
     return a;
 }
 
@@ -465,7 +580,7 @@ trag_status trag_distill_loss_device(const void* d_logits, uint64_t logits_strid
         OpDevice on(who, hip_stream, {d_logits, d_ids, d_teacher, d_counts, d_loss, d_norm, d_row_weight, d_grad, need ? d_work : nullptr});
         if (on.status != TRAG_OK) return on.status;
         const hipStream_t st = (hipStream_t)hip_stream;
-        if (dtype == TRAG_F32) launch_loss<F32>(a, st);
+        if (dtype == TRAG_F32) launch_loss<F32by8>(a, st);
         else if (dtype == TRAG_F16) launch_loss<F16>(a, st);
         else launch_loss<BF16>(a, st);
         return op_launched(who);
@@ -488,7 +603,7 @@ trag_status trag_distill_grad_device(const void* d_logits, uint64_t logits_strid
         OpDevice on(who, hip_stream, {d_logits, d_ids, d_teacher, d_counts, d_norm, d_row_weight, d_grad});
         if (on.status != TRAG_OK) return on.status;
         const hipStream_t st = (hipStream_t)hip_stream;
-        if (dtype == TRAG_F32) launch_grad<F32>(a, st);
+        if (dtype == TRAG_F32) launch_grad<F32by8>(a, st);
         else if (dtype == TRAG_F16) launch_grad<F16>(a, st);
         else launch_grad<BF16>(a, st);
         return op_launched(who);

@@ -24,98 +24,487 @@ struct MmArgs {
     uint32_t m, n, dim;
 };
 
-// 16 bytes of a row from k on, zeros behind its end (a zero on both sides adds nothing)
-__device__ __forceinline__ v4i load_row16(const int8_t* row, uint32_t k, uint32_t dim) {
-    if (k + 16u <= dim) return *reinterpret_cast<const v4i_any*>(row + k);
-    v4i r = {0, 0, 0, 0};
-    if (k < dim) {
+// The end of a row that is not a multiple of the step: a chunk of 16 bytes that would reach over the end is
+// read at dim - 16 instead, in both operands alike (a sum does not mind the order of its terms), and in a the
+// bytes that an earlier chunk has already brought are zero. b is never masked, and nothing is read outside a row.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t k, uint32_t dim) { return min(k, dim - 16u); }
+
+__device__ __forceinline__ v4i load16(const int8_t* p) { return *reinterpret_cast<const v4i_any*>(p); }
+
+// zeros the bytes of a chunk of a that stand for terms before k (the chunk was read at chunk_at(k, dim))
+__device__ __forceinline__ v4i mask_chunk(v4i v, uint32_t k, uint32_t dim) {
+    if (k + 16u <= dim) return v;
+    const uint32_t cut = min(k - (dim - 16u), 16u);
 #pragma unroll
-        for (uint32_t i = 0; i < 16u; ++i)
-            if (k + i < dim) r[i >> 2] |= (int)((uint32_t)(uint8_t)row[k + i] << (8u * (i & 3u)));
+    for (uint32_t w = 0; w < 4u; ++w) {
+        const uint32_t c = cut > 4u * w ? min(cut - 4u * w, 4u) : 0u;
+        v[w] = c == 4u ? 0 : (int)((uint32_t)v[w] & (0xFFFFFFFFu << (8u * c)));
     }
+    return v;
+}
+
+// Rows shorter than a chunk, byte by byte, zeros behind the end.
+__device__ __forceinline__ v4i load_short(const int8_t* row, uint32_t k, uint32_t dim) {
+    v4i r = {0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t i = 0; i < 16u; ++i)
+        if (k + i < dim) r[i >> 2] |= (int)((uint32_t)(uint8_t)row[k + i] << (8u * (i & 3u)));
     return r;
 }
 
 __device__ __forceinline__ float scaled(int acc, float sa, float sb) { return (float)acc * sa * sb; }
 
-// Any alignment, any width: 128 x 128 tile, four waves of 64 x 64, operands through registers into LDS.
-// A row of LDS is 80 bytes: the 16 rows of a fragment read start on 16 different groups of four banks.
-template <typename T>
-__global__ void __launch_bounds__(256) mm_any_kernel(const MmArgs p) {
+// Where the workgroups of a product go: consecutive workgroups land on different dies, each with a cache of its
+// own, so each die gets a run of tiles, walked in columns of GM tiles of a: the tiles a die works on at one
+// time then share rows of both operands.
+struct TilePos {
+    uint32_t m, n;
+    bool there;
+};
+__device__ __forceinline__ TilePos tile_of(uint32_t b, uint32_t m_tiles, uint32_t n_tiles) {
+    constexpr uint32_t GM = 4;
+    const uint32_t tiles = m_tiles * n_tiles, per = (tiles + 7u) / 8u;
+    const uint32_t t = (b & 7u) * per + (b >> 3);
+    if ((b >> 3) >= per || t >= tiles) return {0, 0, false};
+    const uint32_t g = t / (GM * n_tiles), g0 = g * GM, rows = min(GM, m_tiles - g0), in = t - g * GM * n_tiles;
+    return {g0 + in % rows, in / rows, true};
+}
+
+// ---- small tiles, straight into matrix fragments: a wave takes 16 MT rows of a and 16 NT rows of b; lane l holds 16
+// bytes of row l % 16 from k = 16 (l / 16) on, so a wave-instruction reads 64 consecutive bytes of each of 16
+// rows. Nothing goes through LDS but the joining of partial sums where WK waves share one tile's terms, which
+// is what fills the chip when there are few tiles. U: 64-byte steps whose loads are in flight together; the
+// next U are asked for before the current ones are used. WN: tiles side by side in one workgroup.
+template <typename T, int MT, int NT, int WK, int WN, int U, bool SHORT>
+__global__ void __launch_bounds__(64 * WK * WN) mm_direct_kernel(const MmArgs p) {
     typedef typename T::elem E;
-    constexpr int LD = 80;
-    __shared__ __attribute__((aligned(16))) int8_t As[128 * LD];
-    __shared__ __attribute__((aligned(16))) int8_t Bs[128 * LD];
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wid = tid >> 6;
-    const uint32_t m_tiles = (p.m + 127u) / 128u;
-    const uint32_t mt = blockIdx.x % m_tiles, nt = blockIdx.x / m_tiles;
-    const uint32_t m0 = mt * 128u, n0 = nt * 128u;
-    const uint32_t wm = (wid >> 1) * 64u, wn = (wid & 1u) * 64u;
-    const int8_t *ar[2], *br[2];
-    uint32_t kc[2], slot[2];
+    constexpr int FR = MT * NT * 4;   // sums of a lane
+    constexpr int PARTS = WK > 1 ? WK / 2 : 1;
+    __shared__ int part[PARTS][WK > 1 ? WN * FR * 64 : 1];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wid = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t wk = wid % WK, wn = wid / WK;
+    const uint32_t m_tiles = (p.m + 16u * MT - 1u) / (16u * MT);
+    const TilePos at = tile_of(blockIdx.x, m_tiles, (uint32_t)(((uint64_t)p.n + 16u * NT * WN - 1u) / (16u * NT * WN)));
+    if (!at.there) return;   // (the whole workgroup)
+    const uint32_t m0 = at.m * (16u * MT);
+    const uint64_t n0 = ((uint64_t)at.n * WN + wn) * (16u * NT);
+    const uint32_t r16 = lane & 15u, kq = (lane >> 4) * 16u;
+    const uint32_t steps = (p.dim + 63u) / 64u;
+    const uint32_t per = (steps + WK - 1u) / WK;
+    const uint32_t s0 = min(wk * per, steps), s1 = min(s0 + per, steps);
+    const int8_t *ar[MT], *br[NT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const uint32_t c = tid + (uint32_t)i * 256u, r = c >> 2;
-        kc[i] = (c & 3u) * 16u;
-        slot[i] = r * LD + kc[i];
-        ar[i] = p.a + (uint64_t)min(m0 + r, p.m - 1u) * p.lda;
-        br[i] = p.b + (uint64_t)min(n0 + r, p.n - 1u) * p.ldb;
-    }
-    v4i acc[4][4];
+    for (int i = 0; i < MT; ++i) ar[i] = p.a + (uint64_t)min(m0 + (uint32_t)i * 16u + r16, p.m - 1u) * p.lda;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < NT; ++j) br[j] = p.b + min(n0 + (uint32_t)j * 16u + r16, (uint64_t)p.n - 1u) * p.ldb;
+    v4i acc[MT][NT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = v4i{0, 0, 0, 0};
-    v4i fa[2], fb[2];
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) { fa[i] = load_row16(ar[i], kc[i], p.dim); fb[i] = load_row16(br[i], kc[i], p.dim); }
-    for (uint32_t k0 = 0; k0 < p.dim; k0 += 64u) {
-        __syncthreads();
+        for (int j = 0; j < NT; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    v4i fa[2][U][MT], fb[2][U][NT];
+    auto fetch = [&](int buf, uint32_t s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            *reinterpret_cast<v4i*>(As + slot[i]) = fa[i];
-            *reinterpret_cast<v4i*>(Bs + slot[i]) = fb[i];
+        for (int u = 0; u < U; ++u) {
+            if (s + (uint32_t)u >= s1) continue;   // (wave-uniform)
+            const uint32_t k = (s + (uint32_t)u) * 64u + kq;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fb[buf][u][j] = SHORT ? load_short(br[j], k, p.dim) : load16(br[j] + chunk_at(k, p.dim));
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa[buf][u][i] = SHORT ? load_short(ar[i], k, p.dim) : load16(ar[i] + chunk_at(k, p.dim));
         }
-        __syncthreads();
-        if (k0 + 64u < p.dim) {
+    };
+    auto multiply = [&](int buf, uint32_t s) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = load_row16(ar[i], k0 + 64u + kc[i], p.dim);
-                fb[i] = load_row16(br[i], k0 + 64u + kc[i], p.dim);
+        for (int u = 0; u < U; ++u) {
+            if (s + (uint32_t)u >= s1) continue;
+            const bool last = !SHORT && (s + (uint32_t)u + 1u) * 64u > p.dim;
+            const uint32_t k = (s + (uint32_t)u) * 64u + kq;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const v4i x = last ? mask_chunk(fa[buf][u][i], k, p.dim) : fa[buf][u][i];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, fb[buf][u][j], acc[i][j], 0, 0, 0);
             }
         }
-        const uint32_t fr = (lane & 15u) * LD + (lane >> 4) * 16u;
-        v4i xa[4], xb[4];
+    };
+    fetch(0, s0);
+    for (uint32_t s = s0; s < s1; s += 2u * U) {
+        fetch(1, s + U);
+        multiply(0, s);
+        fetch(0, s + 2u * U);
+        multiply(1, s + U);
+    }
+    // the waves' sums joined two by two: half of those left hand theirs over, half add
+    if constexpr (WK > 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            xa[i] = *reinterpret_cast<const v4i*>(As + (wm + (uint32_t)i * 16u) * LD + fr);
-            xb[i] = *reinterpret_cast<const v4i*>(Bs + (wn + (uint32_t)i * 16u) * LD + fr);
+        for (int half = WK / 2; half >= 1; half /= 2) {
+            if (wk >= (uint32_t)half && wk < 2u * half) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) part[wk - half][(wn * FR + (uint32_t)((i * NT + j) * 4 + r)) * 64u + lane] = acc[i][j][r];
+            }
+            __syncthreads();
+            if (wk < (uint32_t)half) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] += part[wk][(wn * FR + (uint32_t)((i * NT + j) * 4 + r)) * 64u + lane];
+            }
+            if (half > 1) __syncthreads();
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+        if (wk > 0) return;
     }
     // lane l holds column l % 16 of rows 4 (l / 16) .. + 3
     E* const out = reinterpret_cast<E*>(p.out);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t col = n0 + wn + (uint32_t)j * 16u + (lane & 15u);
-        const float sb = col < p.n ? (p.sb ? p.sb[col] : 1.0f) : 0.0f;
+    for (int j = 0; j < NT; ++j) {
+        const uint64_t col = n0 + (uint32_t)j * 16u + r16;
+        if (col >= p.n) continue;
+        const float sb = p.sb ? p.sb[col] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint32_t row = m0 + wm + (uint32_t)i * 16u + (lane >> 4) * 4u + (uint32_t)r;
-                if (row < p.m && col < p.n) T::store(out + (uint64_t)row * p.ldo + col, scaled(acc[i][j][r], p.sa ? p.sa[row] : 1.0f, sb));
+                const uint32_t row = m0 + (uint32_t)i * 16u + (lane >> 4) * 4u + (uint32_t)r;
+                if (row < p.m) *(out + (uint64_t)row * p.ldo + col) = T::round(scaled(acc[i][j][r], p.sa ? p.sa[row] : 1.0f, sb));
             }
     }
 }
 
+// ---- tiles through LDS: WM x WN waves of (16 MT) x (16 NT) sums each, 128 bytes of every row a step. Bound by the
+// matrix cores where there are tiles enough. LDS rows are 128 bytes without padding; chunk c of row r stands at
+// slot c ^ (r / 2 % 8), so that the 16 rows of a fragment read fall on different banks.
+// DMA: rows start on 16 bytes. Both operands go from memory straight into LDS (16 bytes a lane, no registers on the
+// way; the permutation is applied to the addresses that the lanes fetch), ST stages deep: a step waits for its own
+// transfers, which were asked for ST - 1 steps earlier, passes one barrier, asks for the transfers of the step
+// that takes the stage just left, and multiplies. Otherwise the same through registers, two stages.
+template <typename T, int WM, int WN, int MT, int NT, int KG, int ST, bool DMA>
+__global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs p) {
+    typedef typename T::elem E;
+    constexpr int NW = WM * WN;
+    constexpr uint32_t BM = 16u * MT * WM, BN = 16u * NT * WN;
+    constexpr uint32_t STAGE = (BM + BN) * 128u;
+    constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // pieces (8 rows, 1 KB) of each operand a wave brings a step
+    static_assert(PA * NW * 8 == (int)BM && PB * NW * 8 == (int)BN, "whole pieces");
+    static_assert(DMA || ST == 2, "through registers: two stages");
+    constexpr uint32_t PER = 16u / sizeof(E);              // elements of 16 bytes
+    constexpr uint32_t RUN = 16u * NT, LDO = RUN + PER;    // a row of a wave's piece of the epilogue
+    static_assert(NW * 16u * LDO * sizeof(E) <= ST * STAGE, "the epilogue's pieces fit the stages");
+    constexpr int FR = MT * NT * 4;                        // sums of a lane
+    static_assert(KG == 1 || KG / 2 * NW * FR * 256 <= (int)(KG * ST * STAGE), "the sums that are handed over fit the stages");
+    __shared__ __attribute__((aligned(1024))) int8_t all[KG * ST * STAGE];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t kg = wave / NW, wid = wave % NW;
+    int8_t* const lds = all + kg * (ST * STAGE);           // (each group of waves has stages of its own)
+    const uint32_t wm = wid / WN, wn = wid % WN;
+    const TilePos at = tile_of(blockIdx.x, (p.m + BM - 1u) / BM, (uint32_t)(((uint64_t)p.n + BN - 1u) / BN));
+    if (!at.there) return;
+    const uint32_t m0 = at.m * BM, n0 = at.n * BN;
+    // the terms are dealt out to the groups in runs; every group passes the same barriers, with or without a step to do
+    const uint32_t total = (p.dim + 127u) / 128u, rounds = (total + KG - 1u) / KG;
+    const uint32_t first = min(kg * rounds, total), steps = min(rounds, total - first);
+    uint32_t oa[PA], ob[PB];                               // byte offsets of a lane's chunks from the tile's first row
+    const uint32_t c8 = (lane & 7u);
+#pragma unroll
+    for (int i = 0; i < PA; ++i) {
+        const uint32_t row = (wid * PA + (uint32_t)i) * 8u + (lane >> 3);
+        oa[i] = (min(m0 + row, p.m - 1u) - m0) * (uint32_t)p.lda + (c8 ^ ((row >> 1) & 7u)) * 16u;
+    }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+        const uint32_t row = (wid * PB + (uint32_t)i) * 8u + (lane >> 3);
+        ob[i] = (min(n0 + row, p.n - 1u) - n0) * (uint32_t)p.ldb + (c8 ^ ((row >> 1) & 7u)) * 16u;
+    }
+    const int8_t* const abase = p.a + (uint64_t)m0 * p.lda;
+    const int8_t* const bbase = p.b + (uint64_t)n0 * p.ldb;
+    // bytes by which a chunk of the last step is moved back to end at the row's end (or 0)
+    auto back = [&](uint32_t step, uint32_t first_row, int i) __attribute__((always_inline)) {
+        const uint32_t row = first_row + (uint32_t)i * 8u + (lane >> 3);
+        const uint32_t k = step * 128u + (c8 ^ ((row >> 1) & 7u)) * 16u;
+        return k - chunk_at(k, p.dim);
+    };
+    typedef __attribute__((address_space(3))) int8_t* lds_ptr;
+    v4i ra[DMA ? 1 : PA], rb[DMA ? 1 : PB];
+    auto transfer = [&](uint32_t slot, uint32_t step) __attribute__((always_inline)) {
+        const int8_t* const sa = abase + (uint64_t)step * 128u;
+        const int8_t* const sb = bbase + (uint64_t)step * 128u;
+        const bool whole = (step + 1u) * 128u <= p.dim;
+        if constexpr (DMA) {
+#if defined(__HIP_DEVICE_COMPILE__)
+            const uint32_t to = (uint32_t)(uintptr_t)(lds_ptr)lds + slot * STAGE;
+            const uint32_t ta = to + wid * (PA * 1024u), tb = to + BM * 128u + wid * (PB * 1024u);
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < PA; ++i) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(ta + (uint32_t)i * 1024u), "v"(oa[i]), "s"(sa) : "memory");
+#pragma unroll
+                for (int i = 0; i < PB; ++i) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(tb + (uint32_t)i * 1024u), "v"(ob[i]), "s"(sb) : "memory");
+            } else {   // (dim is a multiple of 16 here: a chunk is whole, or moved back to the row's last one)
+#pragma unroll
+                for (int i = 0; i < PA; ++i) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(ta + (uint32_t)i * 1024u), "v"(oa[i] - back(step, wid * PA * 8u, i)), "s"(sa) : "memory");
+#pragma unroll
+                for (int i = 0; i < PB; ++i) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(tb + (uint32_t)i * 1024u), "v"(ob[i] - back(step, wid * PB * 8u, i)), "s"(sb) : "memory");
+            }
+#endif
+        } else {
+#pragma unroll
+            for (int i = 0; i < PA; ++i) ra[i] = load16(sa + oa[i] - (whole ? 0u : back(step, wid * PA * 8u, i)));
+#pragma unroll
+            for (int i = 0; i < PB; ++i) rb[i] = load16(sb + ob[i] - (whole ? 0u : back(step, wid * PB * 8u, i)));
+        }
+    };
+    auto put = [&](uint32_t slot) __attribute__((always_inline)) {   // (through registers: what transfer() brought, into LDS)
+        if constexpr (!DMA) {
+            int8_t* const to = lds + slot * STAGE + lane * 16u;
+#pragma unroll
+            for (int i = 0; i < PA; ++i) *reinterpret_cast<v4i*>(to + (wid * PA + (uint32_t)i) * 1024u) = ra[i];
+#pragma unroll
+            for (int i = 0; i < PB; ++i) *reinterpret_cast<v4i*>(to + BM * 128u + (wid * PB + (uint32_t)i) * 1024u) = rb[i];
+        }
+    };
+    v4i acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = v4i{0, 0, 0, 0};
+    const uint32_t r16 = lane & 15u, q = lane >> 4;
+    const uint32_t sw = (r16 >> 1) & 7u;
+    const uint32_t fra = (wm * (16u * MT) + r16) * 128u, frb = BM * 128u + (wn * (16u * NT) + r16) * 128u;
+    auto multiply = [&](uint32_t slot, uint32_t step) __attribute__((always_inline)) {
+        const int8_t* const A = lds + slot * STAGE + fra;
+        const int8_t* const B = lds + slot * STAGE + frb;
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; ++h) {
+            const uint32_t k = step * 128u + h * 64u;
+            if (k >= p.dim) break;
+            const uint32_t c = ((h * 4u + q) ^ sw) * 16u;
+            v4i xa[MT], xb[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) xb[j] = *reinterpret_cast<const v4i*>(B + j * 2048 + c);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xa[i] = *reinterpret_cast<const v4i*>(A + i * 2048 + c);
+            if (k + 64u > p.dim) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) xa[i] = mask_chunk(xa[i], k + q * 16u, p.dim);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+        }
+    };
+    if constexpr (DMA) {
+#pragma unroll
+        for (uint32_t s = 0; s < ST - 1u; ++s)
+            if (s < steps) transfer(s, first + s);
+        uint32_t slot = 0;
+        for (uint32_t s = 0; s < rounds; ++s) {
+            // (in flight behind this step's: those of the next ST - 2, if there are as many)
+            if (ST > 2 && s + (ST - 1u) <= steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (PA + PB)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (s + (ST - 1u) < steps) transfer(slot == 0 ? ST - 1u : slot - 1u, first + s + (ST - 1u));
+            if (KG == 1 || s < steps) multiply(slot, first + s);
+            slot = slot + 1u == ST ? 0u : slot + 1u;
+        }
+    } else {
+        if (KG == 1 || steps) {
+            transfer(0, first);
+            put(0);
+        }
+        for (uint32_t s = 0; s < rounds; ++s) {
+            __syncthreads();
+            if (s + 1u < steps) transfer((s + 1u) & 1u, first + s + 1u);
+            if (KG == 1 || s < steps) multiply(s & 1u, first + s);
+            if (s + 1u < steps) put((s + 1u) & 1u);
+        }
+    }
+    __syncthreads();
+    // the groups' sums joined two by two: half of those left hand theirs over, half add
+    if constexpr (KG > 1) {
+        int* const part = reinterpret_cast<int*>(all);
+#pragma unroll
+        for (uint32_t half = KG / 2; half >= 1u; half /= 2u) {
+            if (kg >= half && kg < 2u * half) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        *reinterpret_cast<v4i*>(part + ((((kg - half) * NW + wid) * (MT * NT) + (uint32_t)(i * NT + j)) * 64u + lane) * 4u) = acc[i][j];
+            }
+            __syncthreads();
+            if (kg < half) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[i][j] += *reinterpret_cast<const v4i*>(part + (((kg * NW + wid) * (MT * NT) + (uint32_t)(i * NT + j)) * 64u + lane) * 4u);
+            }
+            __syncthreads();
+        }
+        if (kg > 0) return;
+    }
+    // 16 rows of the wave's columns at a time through a piece of LDS of its own: a store then covers whole runs of a row
+    E* const out = reinterpret_cast<E*>(p.out);
+    E* const piece = reinterpret_cast<E*>(all) + wid * (16u * LDO);
+    float sb[NT];
+    const uint32_t col0 = n0 + wn * RUN;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const uint32_t col = col0 + (uint32_t)j * 16u + r16;
+        sb[j] = p.sb && col < p.n ? p.sb[col] : 1.0f;
+    }
+    typedef E evec __attribute__((ext_vector_type(16 / sizeof(E)), aligned(sizeof(E))));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const uint32_t row0 = m0 + wm * (16u * MT) + (uint32_t)i * 16u;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t row = row0 + q * 4u + (uint32_t)r;
+            const float sa = p.sa && row < p.m ? p.sa[row] : 1.0f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(piece + (q * 4u + (uint32_t)r) * LDO + (uint32_t)j * 16u + r16) = T::round(scaled(acc[i][j][r], sa, sb[j]));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        constexpr uint32_t LPR = RUN / PER;                // lanes a row
+        constexpr uint32_t RPI = 64u / LPR < 16u ? 64u / LPR : 16u;   // rows a wave-instruction
+#pragma unroll
+        for (uint32_t r = 0; r < 16u; r += RPI) {
+            const uint32_t lr = r + lane / LPR, row = row0 + lr, c = (lane % LPR) * PER;
+            if (lr < 16u && row < p.m) {
+                const E* const from = piece + lr * LDO + c;
+                E* const to = out + (uint64_t)row * p.ldo + col0 + c;
+                if (col0 + c + PER <= p.n) *reinterpret_cast<evec*>(to) = *reinterpret_cast<const evec*>(from);
+                else
+                    for (uint32_t x = 0; x < PER; ++x)
+                        if (col0 + c + x < p.n) to[x] = from[x];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+uint32_t grid8(uint64_t tiles) { return (uint32_t)((tiles + 7u) / 8u * 8u); }   // (a run of tiles for each of 8 dies)
+
+template <typename T, int MT, int NT, int WK, int WN, int U, bool SHORT = false>
+void launch_direct(const MmArgs& p, hipStream_t st) {
+    const uint64_t mt = (p.m + 16u * MT - 1u) / (16u * MT), nt = ((uint64_t)p.n + 16u * NT * WN - 1) / (16u * NT * WN);
+    hipLaunchKernelGGL((mm_direct_kernel<T, MT, NT, WK, WN, U, SHORT>), dim3(grid8(mt * nt)), dim3(64 * WK * WN), 0, st, p);
+}
+
+template <typename T, int WM, int WN, int MT, int NT, int KG, int ST, bool DMA>
+void launch_tile(const MmArgs& p, hipStream_t st) {
+    constexpr uint32_t BM = 16u * MT * WM, BN = 16u * NT * WN;
+    const uint64_t tiles = (uint64_t)((p.m + BM - 1u) / BM) * (((uint64_t)p.n + BN - 1u) / BN);
+    hipLaunchKernelGGL((mm_tile_kernel<T, WM, WN, MT, NT, KG, ST, DMA>), dim3(grid8(tiles)), dim3(64 * WM * WN * KG), 0, st, p);
+}
+
+// Transfers straight into LDS: whole 16-byte chunks at addresses that are multiples of 16.
+bool dma_fits(const MmArgs& p) {
+    return p.dim % 16u == 0 && p.lda % 16u == 0 && p.ldb % 16u == 0 && aligned_to(p.a, 16) && aligned_to(p.b, 16);
+}
+
+// Which tile. Every form gives the same bits, so the choice is one of time alone: the one with the least
+//   2.5 us + max(rounds (fix + per * steps a group of waves does), bytes the tiles read / rate + output / 5 TB/s),
+// rounds = tiles over what 256 CUs hold at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
+// up. The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
+//   16 x 4096 x 4096   16 x 64 tiles in 4 groups   7.2    in 1   14.7 (n 16384)   32 x 64 in 4   8.2
+//   64 x 4096 x 4096   32 x 64 in 4   8.8    64 x 64 in 2  10.9    in 1  15.6
+//   256 x 4096 x 4096  64 x 64 in 2  11.6    128 x 128 in 2  21.7    in 1  33.1    256 x 256  50
+//   1024 x 4096 x 4096 128 x 128 in 2  23.7    64 x 64 in 1  29.5    128 x 128 in 1  34.4    256 x 256  51
+//   4096 x 16384 x 4096  256 x 256  239    128 x 128 in 1  355
+//   1 x 1M x 384  16 x 64 in 1  69    64 x 1M x 384  64 x 128  114, 64 x 64  127    128 x 1M x 384  128 x 128  179, 64 x 64  235
+// and for rows at any byte (through registers):
+//   30 x 50021 x 777  32 x 64  12.6, 64 x 64  13.4    512 x 4096 x 4001  64 x 64  27.8, 64 x 128  33.0
+//   1024 x 4096 x 4001  64 x 128  36.9, 128 x 128  42.6    4096 x 8192 x 4001  256 x 256  157, 128 x 128  223
+enum TileForm { T16, T16G4, T32, T32G4, T64, T64G2, T64G4, T64x128, T128, T128G2, T256, N_FORMS };
+struct FormCost {
+    uint16_t bm, bn, groups, threads;
+    uint16_t held;             // workgroups a CU holds (0: this form is not built)
+    float fix, lo, hi;
+};
+constexpr FormCost DMA_COST[N_FORMS] = {
+    {16, 64, 1, 128, 5, 4.0f, 0.30f, 0.38f},   {16, 64, 4, 512, 1, 2.5f, 0.28f, 0.30f}, {32, 64, 1, 128, 6, 5.5f, 0.45f, 0.50f},
+    {32, 64, 4, 512, 1, 2.2f, 0.50f, 0.55f},   {64, 64, 1, 256, 5, 3.5f, 0.36f, 0.73f}, {64, 64, 2, 512, 1, 2.3f, 0.42f, 0.43f},
+    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.5f, 0.55f, 1.0f}, {128, 128, 1, 256, 2, 5.0f, 0.60f, 1.25f},
+    {128, 128, 2, 512, 1, 6.5f, 0.85f, 0.92f}, {256, 256, 1, 512, 1, 8.5f, 1.30f, 1.60f}};
+constexpr FormCost ANY_COST[N_FORMS] = {
+    {16, 64, 1, 128, 8, 3.0f, 0.43f, 0.60f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},   {32, 64, 1, 128, 6, 3.0f, 0.48f, 0.80f},
+    {32, 64, 4, 512, 1, 2.5f, 1.05f, 1.15f},   {64, 64, 1, 256, 5, 2.0f, 0.58f, 1.60f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
+    {64, 64, 4, 1024, 1, 2.0f, 1.50f, 1.60f},  {64, 128, 1, 256, 3, 3.0f, 0.80f, 1.45f}, {128, 128, 1, 256, 2, 4.0f, 0.90f, 1.60f},
+    {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},   {256, 256, 1, 512, 1, 7.0f, 1.80f, 2.20f}};
+
+int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
+    constexpr double CUS = 256.0;
+    const double steps = (double)((p.dim + 127u) / 128u);
+    int best = T256;
+    double least = 1e300;
+    for (int f = 0; f < N_FORMS; ++f) {
+        const FormCost& c = dma ? DMA_COST[f] : ANY_COST[f];
+        if (!c.held) continue;
+        const double tiles = (double)((p.m + c.bm - 1u) / c.bm) * (double)(((uint64_t)p.n + c.bn - 1u) / c.bn);
+        if ((tiles + 8.0) * c.threads >= 4294967296.0) continue;   // (a grid's threads are counted in 32 bits)
+        const double at_once = CUS * c.held, full = tiles < at_once ? tiles / at_once : 1.0;
+        const double rounds = __builtin_ceil(tiles / at_once);
+        const double busy = rounds * (c.fix + (c.lo + (c.hi - c.lo) * full) * __builtin_ceil(steps / c.groups));
+        const double moved = tiles * (c.bm + c.bn) * (double)p.dim / (dma ? 8.0e6 : 6.5e6) + (double)p.m * p.n * out_bytes / 5.0e6;
+        const double t = busy > moved ? busy : moved;
+        if (t < least) {
+            least = t;
+            best = f;
+        }
+    }
+    return best;
+}
+
 template <typename T>
 void launch_mm(const MmArgs& p, hipStream_t st) {
-    const uint64_t tiles = (uint64_t)((p.m + 127u) / 128u) * ((p.n + 127u) / 128u);
-    hipLaunchKernelGGL((mm_any_kernel<T>), dim3((uint32_t)tiles), dim3(256), 0, st, p);
+    if (p.dim < 16u) return launch_direct<T, 1, 8, 1, 4, 1, true>(p, st);
+    // (the tiles' offsets from their first row are 32 bits, over 255 rows at most)
+    if (p.lda >= (1u << 24) || p.ldb >= (1u << 24)) return launch_direct<T, 4, 1, 8, 1, 2>(p, st);
+    const bool dma = dma_fits(p);
+    // Few rows of a, short b, long rows at any byte: a wave's fragments straight from memory, eight waves a tile's terms
+    // (16 x 4096 x 4001: 7.4 us, the tiles 11.9; 30 x 2000 x 4001: 9.7, the tiles 13.5; aligned rows have the tiles ahead).
+    if (!dma && p.m <= 64u && p.n <= 8192u && p.dim >= 1024u) {
+        if (p.m <= 16u) return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
+        return launch_direct<T, 4, 1, 8, 1, 2>(p, st);
+    }
+    const int form = choose_form(p, dma, sizeof(typename T::elem));
+    if (dma) {
+        switch (form) {
+            case T16: return launch_tile<T, 1, 2, 1, 2, 1, 2, true>(p, st);
+            case T16G4: return launch_tile<T, 1, 2, 1, 2, 4, 3, true>(p, st);
+            case T32: return launch_tile<T, 1, 2, 2, 2, 1, 2, true>(p, st);
+            case T32G4: return launch_tile<T, 1, 2, 2, 2, 4, 3, true>(p, st);
+            case T64: return launch_tile<T, 2, 2, 2, 2, 1, 2, true>(p, st);
+            case T64G2: return launch_tile<T, 2, 2, 2, 2, 2, 4, true>(p, st);
+            case T64x128: return launch_tile<T, 2, 2, 2, 4, 1, 2, true>(p, st);
+            case T128: return launch_tile<T, 2, 2, 4, 4, 1, 2, true>(p, st);
+            case T128G2: return launch_tile<T, 2, 2, 4, 4, 2, 2, true>(p, st);
+            default: return launch_tile<T, 4, 2, 4, 8, 1, 2, true>(p, st);
+        }
+    }
+    switch (form) {
+        case T16: return launch_tile<T, 1, 2, 1, 2, 1, 2, false>(p, st);
+        case T32: return launch_tile<T, 1, 2, 2, 2, 1, 2, false>(p, st);
+        case T32G4: return launch_tile<T, 1, 2, 2, 2, 4, 2, false>(p, st);
+        case T64: return launch_tile<T, 2, 2, 2, 2, 1, 2, false>(p, st);
+        case T64G4: return launch_tile<T, 2, 2, 2, 2, 4, 2, false>(p, st);
+        case T64x128: return launch_tile<T, 2, 2, 2, 4, 1, 2, false>(p, st);
+        case T128: return launch_tile<T, 2, 2, 4, 4, 1, 2, false>(p, st);
+        default: return launch_tile<T, 4, 2, 4, 8, 1, 2, false>(p, st);
+    }
 }
 
 }  // namespace
@@ -136,9 +525,9 @@ extern "C" trag_status trag_matmul_q8_device(const int8_t* d_a, uint64_t a_strid
         if (!aligned_to(d_a_scale, 4) || !aligned_to(d_b_scale, 4) || !aligned_to(d_out, dtype_bytes(out_dtype)))
             return bad("an array is not aligned to its elements");
         if (dim > DIM_MAX) return set_error(TRAG_UNSUPPORTED, std::string(who) + ": a sum of more than 131071 products can pass 32 bits");
-        // (a grid is at most 2^32 threads: 2^24 tiles of 128 x 128)
-        if ((((uint64_t)m + 127) / 128) * (((uint64_t)n + 127) / 128) >= (1ull << 24))
-            return set_error(TRAG_UNSUPPORTED, std::string(who) + ": the product has 2^24 tiles of 128 x 128 or more: split it");
+        // (a grid's threads are counted in 32 bits)
+        if ((((uint64_t)m + 127) / 128) * (((uint64_t)n + 127) / 128) >= (1ull << 22))
+            return set_error(TRAG_UNSUPPORTED, std::string(who) + ": the product has 2^22 tiles of 128 x 128 or more: split it");
         OpDevice on(who, hip_stream, {d_a, d_a_scale, d_b, d_b_scale, d_out});
         if (on.status != TRAG_OK) return on.status;
         const MmArgs p{d_a, d_b, d_a_scale, d_b_scale, d_out, a_stride, b_stride, out_stride, m, n, dim};

@@ -14,69 +14,43 @@ namespace trag {
 inline uint32_t dtype_bytes(uint32_t dtype) { return dtype == TRAG_F32 ? 4u : 2u; }
 inline bool aligned_to(const void* p, uint32_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
 
-// ---- element types: 8 consecutive elements as floats. A caller's rows may start at any element (odd widths,
-// odd strides), so the wide accesses ask for element alignment only; the hardware serves unaligned 16-byte
-// accesses, and an aligned row pays nothing for it.
+// ---- element types, W consecutive elements (16 bytes) at a time. A caller's rows may start at any element (odd
+// widths, odd strides), so the wide accesses ask for element alignment only; the hardware serves unaligned 16-byte
+// accesses, and an aligned row pays nothing for it. `round`: a result is rounded to f32 and then to the type.
 struct F32 {
     typedef float elem;
-    typedef float vec4 __attribute__((ext_vector_type(4), aligned(4)));
-    static __device__ __forceinline__ float load(const elem* p) { return *p; }
-    static __device__ __forceinline__ void store(elem* p, float v) { *p = v; }
-    static __device__ __forceinline__ void load8(const elem* p, float (&v)[8]) {
-        const vec4 a = *reinterpret_cast<const vec4*>(p), b = *reinterpret_cast<const vec4*>(p + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-    }
-    static __device__ __forceinline__ void store8(elem* p, const float (&v)[8]) {
-        vec4 a, b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { a[i] = v[i]; b[i] = v[4 + i]; }
-        *reinterpret_cast<vec4*>(p) = a;
-        *reinterpret_cast<vec4*>(p + 4) = b;
-    }
+    static constexpr int W = 4;
+    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+    static __device__ __forceinline__ float round(float v) { return v; }
 };
-
 struct F16 {
-    // A result is rounded to f32 and then to f16, as in the other types: the product in front of the conversion is hidden
-    // from the compiler, which would fold the two into a mixed-precision multiply with a single rounding.
+    typedef _Float16 elem;
+    static constexpr int W = 8;
+    typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    // (the value is hidden from the compiler, which would fold a product and its conversion into a mixed-precision
+    // multiply with a single rounding)
     static __device__ __forceinline__ _Float16 round(float v) {
         asm("" : "+v"(v));
         return (_Float16)v;
     }
-    typedef _Float16 elem;
-    typedef _Float16 vec8 __attribute__((ext_vector_type(8), aligned(2)));
-    static __device__ __forceinline__ float load(const elem* p) { return (float)*p; }
-    static __device__ __forceinline__ void store(elem* p, float v) { *p = round(v); }
-    static __device__ __forceinline__ void load8(const elem* p, float (&v)[8]) {
-        const vec8 a = *reinterpret_cast<const vec8*>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-    }
-    static __device__ __forceinline__ void store8(elem* p, const float (&v)[8]) {
-        vec8 a;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = round(v[i]);
-        *reinterpret_cast<vec8*>(p) = a;
-    }
 };
-
 struct BF16 {
     typedef __bf16 elem;
-    typedef __bf16 vec8 __attribute__((ext_vector_type(8), aligned(2)));
-    static __device__ __forceinline__ float load(const elem* p) { return (float)*p; }
-    static __device__ __forceinline__ void store(elem* p, float v) { *p = (__bf16)v; }
-    static __device__ __forceinline__ void load8(const elem* p, float (&v)[8]) {
-        const vec8 a = *reinterpret_cast<const vec8*>(p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)a[i];
-    }
-    static __device__ __forceinline__ void store8(elem* p, const float (&v)[8]) {
-        vec8 a;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = (__bf16)v[i];
-        *reinterpret_cast<vec8*>(p) = a;
-    }
+    static constexpr int W = 8;
+    typedef __bf16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    static __device__ __forceinline__ __bf16 round(float v) { return (__bf16)v; }
 };
+template <typename T>
+__device__ __forceinline__ typename T::vec load_vec(const typename T::elem* p) { return *reinterpret_cast<const typename T::vec*>(p); }
+template <typename T>
+__device__ __forceinline__ void store_vec(typename T::elem* p, typename T::vec v) { *reinterpret_cast<typename T::vec*>(p) = v; }
+template <typename T>
+__device__ __forceinline__ typename T::vec fill_vec(float v) {
+    typename T::vec r;
+#pragma unroll
+    for (int i = 0; i < T::W; ++i) r[i] = T::round(v);
+    return r;
+}
 
 // ---- entry points without a handle. The device is the stream's; for the default stream it is the one the
 // arrays live on. Arrays that are not device memory of that device are refused on the host: a kernel would fault.

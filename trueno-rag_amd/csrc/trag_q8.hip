@@ -12,7 +12,7 @@
 // roundings; with them it is a function of the inputs alone.
 //
 // Bound by HBM: per element a read of x (and the residual), a write of the sum, of q and, if asked for, of
-// the values they stand for. One wave a row up to 1024 elements, one workgroup a row beyond; a row too
+// the values they stand for. 16 lanes to a wave a row up to 2048 elements, one workgroup a row beyond; a row too
 // long for registers (over 32768 elements) is read twice, the second time from the caches.
 #include "trag_ops.h"
 
@@ -32,8 +32,6 @@ struct Q8Args {
     float eps;
 };
 
-typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
-
 // nearest(127 p / top), ties to even. inv = 127 / top has its own rounding, which could move a tie off the
 // middle (or onto it): next to a border the side is taken from 127 p against the border times top.
 __device__ __forceinline__ int q8_nearest(double p, double inv, double top) {
@@ -48,83 +46,87 @@ __device__ __forceinline__ int q8_nearest(double p, double inv, double top) {
     return (int)r;
 }
 
-template <typename T, bool NORM>
-__device__ __forceinline__ void load_products(const Q8Args& a, const typename T::elem* x, const typename T::elem* res,
-                                              const typename T::elem* w, typename T::elem* sum, uint32_t e, bool write_sum,
-                                              double (&p)[8], double& ss) {
-    float xv[8], rv[8], wv[8];
-    const bool full = e + 8u <= a.dim;
-    if (full) {
-        T::load8(x + e, xv);
-        if (NORM && res) T::load8(res + e, rv);
-        if (NORM && w) T::load8(w + e, wv);
+// h w of N consecutive elements (W, or one behind the last whole vector); h goes to the sum's array and into the row's sum
+// of squares
+template <typename T, bool NORM, int N>
+__device__ __forceinline__ void products(const typename T::elem* x, const typename T::elem* res, const typename T::elem* w,
+                                         typename T::elem* sum, uint32_t e, double (&p)[N], double& ss) {
+    typedef typename T::elem E;
+    E xv[N], rv[N], wv[N];
+    if constexpr (N == T::W) {
+        const typename T::vec v = load_vec<T>(x + e);
+#pragma unroll
+        for (int i = 0; i < N; ++i) xv[i] = v[i];
+        if (NORM && res) {
+            const typename T::vec r = load_vec<T>(res + e);
+#pragma unroll
+            for (int i = 0; i < N; ++i) rv[i] = r[i];
+        }
+        if (NORM && w) {
+            const typename T::vec u = load_vec<T>(w + e);
+#pragma unroll
+            for (int i = 0; i < N; ++i) wv[i] = u[i];
+        }
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const bool in = e + (uint32_t)i < a.dim;
-            xv[i] = in ? T::load(x + e + i) : 0.0f;
-            if (NORM && res) rv[i] = in ? T::load(res + e + i) : 0.0f;
-            if (NORM && w) wv[i] = in ? T::load(w + e + i) : 0.0f;
-        }
+        xv[0] = x[e];
+        if (NORM && res) rv[0] = res[e];
+        if (NORM && w) wv[0] = w[e];
     }
-    if (NORM && sum && write_sum) {
-        float sv[8];
+    if (NORM && sum) {
+        typename T::vec s;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sv[i] = res ? xv[i] + rv[i] : xv[i];
-        if (full) T::store8(sum + e, sv);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (e + (uint32_t)i < a.dim) T::store(sum + e + i, sv[i]);
-        }
+        for (int i = 0; i < N; ++i) s[i] = T::round(res ? (float)xv[i] + (float)rv[i] : (float)xv[i]);
+        if constexpr (N == T::W) store_vec<T>(sum + e, s);
+        else sum[e] = s[0];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        double h = (double)xv[i];
-        if (NORM && res) h += (double)rv[i];
-        p[i] = (NORM && w) ? h * (double)wv[i] : h;
+    for (int i = 0; i < N; ++i) {
+        double h = (double)(float)xv[i];
+        if (NORM && res) h += (double)(float)rv[i];
+        p[i] = (NORM && w) ? h * (double)(float)wv[i] : h;
         if (NORM) ss = __builtin_fma(h, h, ss);
         ss = __builtin_fma(p[i], 0.0, ss);   // (NaN as soon as a product is not finite; the maximum alone would pass over a NaN)
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_row8(const Q8Args& a, int8_t* q8, typename T::elem* values, uint32_t e,
-                                           const double (&p)[8], double inv, double top, float scale) {
-    int q[8];
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+template <typename T, int N>
+__device__ __forceinline__ void store_q8(int8_t* q8, typename T::elem* values, uint32_t e, const double (&p)[N], double inv, double top, float scale) {
+    int q[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = inv > 0.0 ? q8_nearest(p[i], inv, top) : 0;
-    if (e + 8u <= a.dim) {
-        u32x2_any o;
+    for (int i = 0; i < N; ++i) q[i] = inv > 0.0 ? q8_nearest(p[i], inv, top) : 0;
+    if constexpr (N == T::W) {
+        uint32_t o[N / 4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < N / 4; ++h)
             o[h] = (uint32_t)(q[4 * h] & 255) | (uint32_t)(q[4 * h + 1] & 255) << 8 | (uint32_t)(q[4 * h + 2] & 255) << 16 |
                    (uint32_t)q[4 * h + 3] << 24;
-        *reinterpret_cast<u32x2_any*>(q8 + e) = o;
+        if constexpr (N == 8) *reinterpret_cast<u32x2_any*>(q8 + e) = u32x2_any{o[0], o[1]};
+        else *reinterpret_cast<u32_any*>(q8 + e) = o[0];
         if (values) {
-            float v[8];
+            typename T::vec v;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (float)q[i] * scale;
-            T::store8(values + e, v);
+            for (int i = 0; i < N; ++i) v[i] = T::round((float)q[i] * scale);
+            store_vec<T>(values + e, v);
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (e + (uint32_t)i < a.dim) {
-                q8[e + i] = (int8_t)q[i];
-                if (values) T::store(values + e + i, (float)q[i] * scale);
-            }
+        q8[e] = (int8_t)q[0];
+        if (values) values[e] = T::round((float)q[0] * scale);
     }
 }
 
-__device__ __forceinline__ double wave_max_f64(double v) {
+template <int L>
+__device__ __forceinline__ double lanes_max(double v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = __builtin_fmax(v, __shfl_xor(v, o));
+    for (int o = L / 2; o > 0; o >>= 1) v = __builtin_fmax(v, __shfl_xor(v, o));
     return v;
 }
-__device__ __forceinline__ double wave_sum_f64(double v) {
+template <int L>
+__device__ __forceinline__ double lanes_sum(double v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
@@ -138,18 +140,25 @@ __device__ __forceinline__ void row_scale(const Q8Args& a, double top, double ss
     scale = fine ? (float)s : __builtin_nanf("");
 }
 
-// NT threads a row (64: a wave a row, four rows a workgroup), NV vectors of eight elements a thread.
-// NV == 0: the row does not fit, it is read again for the integers.
+// NT threads a row (16 lanes, a wave, or a workgroup), NV vectors of W elements a thread; the elements behind the last whole
+// vector: one each for the first few threads. NV == 0: the row does not fit the registers, it is read again for the
+// integers. (Tried: loads without a branch in front -- clamped to the row's last vector, results masked -- and the next
+// row's loads ahead of this row's work. Both need the raw vectors held beside the products, 152 registers instead of 84,
+// and what the occupancy loses is more: 16384 x 4096 bf16 130 us instead of 112, 1M x 384 f32 736 instead of 614.)
 template <typename T, bool NORM, int NT, int NV>
-__global__ void __launch_bounds__(NT == 64 ? 256 : NT) q8_rows_kernel(const Q8Args a) {
+__global__ void __launch_bounds__(NT < 256 ? 256 : NT) q8_rows_kernel(const Q8Args a) {
     typedef typename T::elem E;
-    constexpr int NW = NT / 64;
-    constexpr uint32_t RPB = NT == 64 ? 4u : 1u;
+    static_assert(NT <= 64 || NT >= 256, "a row is a part of a wave, a wave or a workgroup");
+    constexpr int NW = NT / 64, W = T::W;
+    constexpr int L = NT < 64 ? NT : 64;                   // lanes that reduce together
+    constexpr uint32_t RPB = NT < 256 ? 256u / NT : 1u;    // rows a workgroup has at a time
     __shared__ double sh[2][NW > 1 ? NW : 1][2];
-    const uint32_t t = NT == 64 ? threadIdx.x & 63u : threadIdx.x;
+    const uint32_t t = threadIdx.x % (NT < 256 ? NT : 1024);
     const E* const w = reinterpret_cast<const E*>(a.weight);
+    const uint32_t whole = a.dim / W * W, et = whole + t;
+    const bool tail = t < (uint32_t)W && et < a.dim;
     uint32_t turn = 0;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + (NT == 64 ? threadIdx.x >> 6 : 0u); row < a.n_rows;
+    for (uint64_t row = (uint64_t)blockIdx.x * RPB + (NT < 256 ? threadIdx.x / NT : 0u); row < a.n_rows;
          row += (uint64_t)gridDim.x * RPB, turn ^= 1u) {
         const E* const x = reinterpret_cast<const E*>(a.x) + row * a.x_stride;
         const E* const res = a.residual ? reinterpret_cast<const E*>(a.residual) + row * a.residual_stride : nullptr;
@@ -157,26 +166,30 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) q8_rows_kernel(const Q8Ar
         E* const values = a.values ? reinterpret_cast<E*>(a.values) + row * a.values_stride : nullptr;
         int8_t* const q8 = a.q8 + row * a.q8_stride;
         double top = 0.0, ss = 0.0;
-        double p[NV > 0 ? NV : 1][8];
+        double p[NV > 0 ? NV : 1][W], pt[1] = {0.0};
         if constexpr (NV > 0) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const uint32_t e = ((uint32_t)v * NT + t) * 8u;
-                if (e < a.dim) {
-                    load_products<T, NORM>(a, x, res, w, sum, e, true, p[v], ss);
+                const uint32_t e = ((uint32_t)v * NT + t) * W;
+                if (e < whole) {
+                    products<T, NORM, W>(x, res, w, sum, e, p[v], ss);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = __builtin_fmax(top, __builtin_fabs(p[v][i]));
+                    for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[v][i]));
                 }
             }
+            if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, ss);
         } else {
-            for (uint64_t e = t * 8u; e < a.dim; e += NT * 8u) {
-                load_products<T, NORM>(a, x, res, w, sum, (uint32_t)e, false, p[0], ss);
+            // (the sum is written in the second pass: it may go in place of an operand)
+            for (uint32_t e = t * W; e < whole; e += NT * W) {
+                products<T, NORM, W>(x, res, w, nullptr, e, p[0], ss);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = __builtin_fmax(top, __builtin_fabs(p[0][i]));
+                for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[0][i]));
             }
+            if (tail) products<T, NORM, 1>(x, res, w, nullptr, et, pt, ss);
         }
-        top = wave_max_f64(top);
-        ss = wave_sum_f64(ss);
+        top = __builtin_fmax(top, __builtin_fabs(pt[0]));
+        top = lanes_max<L>(top);
+        ss = lanes_sum<L>(ss);
         if constexpr (NW > 1) {
             // (two turns of the array: a wave that is ahead writes the next row's partials beside the ones still read)
             if ((threadIdx.x & 63u) == 0) { sh[turn][threadIdx.x >> 6][0] = top; sh[turn][threadIdx.x >> 6][1] = ss; }
@@ -193,34 +206,45 @@ __global__ void __launch_bounds__(NT == 64 ? 256 : NT) q8_rows_kernel(const Q8Ar
         if constexpr (NV > 0) {
 #pragma unroll
             for (int v = 0; v < NV; ++v) {
-                const uint32_t e = ((uint32_t)v * NT + t) * 8u;
-                if (e < a.dim) store_row8<T>(a, q8, values, e, p[v], inv, top, scale);
+                const uint32_t e = ((uint32_t)v * NT + t) * W;
+                if (e < whole) store_q8<T, W>(q8, values, e, p[v], inv, top, scale);
             }
         } else {
-            for (uint64_t e = t * 8u; e < a.dim; e += NT * 8u) {
-                double again = 0.0;
-                load_products<T, NORM>(a, x, res, w, sum, (uint32_t)e, true, p[0], again);
-                store_row8<T>(a, q8, values, (uint32_t)e, p[0], inv, top, scale);
+            double again = 0.0;
+            for (uint32_t e = t * W; e < whole; e += NT * W) {
+                products<T, NORM, W>(x, res, w, sum, e, p[0], again);
+                store_q8<T, W>(q8, values, e, p[0], inv, top, scale);
             }
+            if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, again);
         }
+        if (tail) store_q8<T, 1>(q8, values, et, pt, inv, top, scale);
     }
 }
 
+// NV: vectors of eight elements, whatever the type
 template <typename T, bool NORM, int NT, int NV>
 void launch_one(const Q8Args& a, hipStream_t st) {
-    const uint32_t rpb = NT == 64 ? 4u : 1u;
+    constexpr uint32_t rpb = NT < 256 ? 256u / NT : 1u, most = 1u << 20;
     const uint64_t blocks = ((uint64_t)a.n_rows + rpb - 1) / rpb;
-    const uint32_t grid = (uint32_t)(blocks < (1u << 20) ? blocks : (1u << 20));
-    hipLaunchKernelGGL((q8_rows_kernel<T, NORM, NT, NV>), dim3(grid), dim3(NT == 64 ? 256 : NT), 0, st, a);
+    const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
+    hipLaunchKernelGGL((q8_rows_kernel<T, NORM, NT, NV * 8 / T::W>), dim3(grid), dim3(NT < 256 ? 256 : NT), 0, st, a);
 }
 
 template <typename T, bool NORM>
 void launch_type(const Q8Args& a, hipStream_t st) {
-    if (a.dim <= 512u) launch_one<T, NORM, 64, 1>(a, st);
+    // As few lanes a row as hold it: more bytes of a lane in flight, fewer steps of the reductions. us, by lanes a row:
+    // 300k x 384 bf16 norm 16 lanes 185, 32 235, 64 350; 200k x 768 bf16 norm 32 lanes 241, 64 299; 30k x 1500 bf16 norm
+    // 64 lanes 86, 256 112-128; 16384 x 4096 bf16 norm 256 threads 112, 512 182.
+    if (a.dim <= 128u) launch_one<T, NORM, 16, 1>(a, st);
+    else if (a.dim <= 256u) launch_one<T, NORM, 16, 2>(a, st);
+    else if (a.dim <= 384u) launch_one<T, NORM, 16, 3>(a, st);
+    else if (a.dim <= 512u) launch_one<T, NORM, 32, 2>(a, st);
+    else if (a.dim <= 768u) launch_one<T, NORM, 32, 3>(a, st);
     else if (a.dim <= 1024u) launch_one<T, NORM, 64, 2>(a, st);
-    else if (a.dim <= 2048u) launch_one<T, NORM, 256, 1>(a, st);
+    else if (a.dim <= 1536u) launch_one<T, NORM, 64, 3>(a, st);
+    else if (a.dim <= 2048u) launch_one<T, NORM, 64, 4>(a, st);
     else if (a.dim <= 4096u) launch_one<T, NORM, 256, 2>(a, st);
-    else if (a.dim <= 8192u) launch_one<T, NORM, 512, 2>(a, st);
+    else if (a.dim <= 8192u) launch_one<T, NORM, 256, 4>(a, st);
     else if (a.dim <= 16384u) launch_one<T, NORM, 1024, 2>(a, st);
     else if (a.dim <= 32768u) launch_one<T, NORM, 1024, 4>(a, st);
     else launch_one<T, NORM, 1024, 0>(a, st);
