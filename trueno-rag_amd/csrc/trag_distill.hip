@@ -31,7 +31,7 @@ struct F32by8 {
 constexpr uint32_t LIST_MAX = 1024;        // teacher entries per row
 constexpr uint32_t ROW_MAX = 65536;        // columns of the row kernel
 constexpr uint32_t PART_STEP = 2048;       // a chunk of a long row is a multiple of this
-constexpr uint32_t PART_MAX = 16384;
+constexpr uint32_t PART_MAX = 8192;        // (gradient of 4096 x 32000 bf16: 111 us, with 16384 117, with 32768 124)
 
 struct DistillArgs {
     const void* z;
@@ -497,9 +497,14 @@ void launch_grad(const DistillArgs& a, hipStream_t st) {
 template <typename T>
 void launch_loss(DistillArgs a, hipStream_t st) {
     if (a.n_cols <= ROW_MAX) {
+        // The fewest threads that hold the row, where there are rows enough to fill the chip (4096 x 4000 bf16 with the gradient:
+        // one wave a row 20.7 us, four 27.5; 64 x 4000: 8.1 and 6.7; 4096 x 32000: four waves 111 us, eight 164, sixteen 346).
+        const bool many = a.n_rows >= 1024u;
         if (a.n_cols <= 512u) launch_row<T, 64, 1>(a, st);
         else if (a.n_cols <= 1024u) launch_row<T, 64, 2>(a, st);
+        else if (a.n_cols <= 2048u && many) launch_row<T, 64, 4>(a, st);
         else if (a.n_cols <= 2048u) launch_row<T, 128, 2>(a, st);
+        else if (a.n_cols <= 4096u && many) launch_row<T, 64, 8>(a, st);
         else if (a.n_cols <= 4096u) launch_row<T, 256, 2>(a, st);
         else if (a.n_cols <= 8192u) launch_row<T, 256, 4>(a, st);
         else if (a.n_cols <= 16384u) launch_row<T, 256, 8>(a, st);

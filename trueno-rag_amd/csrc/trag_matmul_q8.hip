@@ -182,11 +182,15 @@ __global__ void __launch_bounds__(64 * WK * WN) mm_direct_kernel(const MmArgs p)
 // matrix cores where there are tiles enough. LDS rows are 128 bytes without padding; chunk c of row r stands at
 // slot c ^ (r / 2 % 8), so that the 16 rows of a fragment read fall on different banks.
 // DMA: rows start on 16 bytes. Both operands go from memory straight into LDS (16 bytes a lane, no registers on the
-// way; the permutation is applied to the addresses that the lanes fetch), ST stages deep: a step waits for its own
-// transfers, which were asked for ST - 1 steps earlier, passes one barrier, asks for the transfers of the step
-// that takes the stage just left, and multiplies. Otherwise the same through registers, two stages.
+// way; the permutation is applied to the addresses that the lanes fetch), ST stages deep. Otherwise the same through
+// registers, two stages.
+// KG: groups of waves that share a tile's terms, each with stages of its own, where there are few tiles.
+// What bounds it (4096 x 16384 x 4096, 242 us, 2.27 POP/s; 8192 x 8192 x 8192 442 us, 2.49): the matrix cores at the 2.0 GHz
+// that they hold under this load are half busy, fragment reads 22 % of LDS's cycles; reading fragments ahead of the
+// multiplications (128 x 128 tiles 355 -> 303 us) and moving the transfers within a step do not change the largest tile's time.
+// A plain large 8-bit library product takes 288 and 527 us for the two.
 template <typename T, int WM, int WN, int MT, int NT, int KG, int ST, bool DMA>
-__global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs p) {
+__global__ void __launch_bounds__(64 * WM * WN * KG, 2) mm_tile_kernel(const MmArgs p) {
     typedef typename T::elem E;
     constexpr int NW = WM * WN;
     constexpr uint32_t BM = 16u * MT * WM, BN = 16u * NT * WN;
@@ -194,6 +198,9 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
     constexpr int PA = BM / 8 / NW, PB = BN / 8 / NW;      // pieces (8 rows, 1 KB) of each operand a wave brings a step
     static_assert(PA * NW * 8 == (int)BM && PB * NW * 8 == (int)BN, "whole pieces");
     static_assert(DMA || ST == 2, "through registers: two stages");
+    // (through registers the largest tile has none left for a second set of fragments: 110 of them would spill, 414 us
+    // instead of 157 for 4096 x 8192 x 4001)
+    constexpr bool AHEAD = DMA || MT * NT <= 16;
     constexpr uint32_t PER = 16u / sizeof(E);              // elements of 16 bytes
     constexpr uint32_t RUN = 16u * NT, LDO = RUN + PER;    // a row of a wave's piece of the epilogue
     static_assert(NW * 16u * LDO * sizeof(E) <= ST * STAGE, "the epilogue's pieces fit the stages");
@@ -260,6 +267,15 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
             for (int i = 0; i < PB; ++i) rb[i] = load16(sb + ob[i] - (whole ? 0u : back(step, wid * PB * 8u, i)));
         }
     };
+    auto piece = [&](uint32_t slot, uint32_t step, int x) __attribute__((always_inline)) {   // one instruction of a whole step's transfer
+#if defined(__HIP_DEVICE_COMPILE__)
+        const uint32_t to = (uint32_t)(uintptr_t)(lds_ptr)lds + slot * STAGE;
+        if (x < PA)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + (wid * PA + (uint32_t)x) * 1024u), "v"(oa[x < PA ? x : 0]), "s"(abase + (uint64_t)step * 128u) : "memory");
+        else
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to + BM * 128u + (wid * PB + (uint32_t)(x - PA)) * 1024u), "v"(ob[x < PA ? 0 : x - PA]), "s"(bbase + (uint64_t)step * 128u) : "memory");
+#endif
+    };
     auto put = [&](uint32_t slot) __attribute__((always_inline)) {   // (through registers: what transfer() brought, into LDS)
         if constexpr (!DMA) {
             int8_t* const to = lds + slot * STAGE + lane * 16u;
@@ -277,55 +293,104 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
     const uint32_t r16 = lane & 15u, q = lane >> 4;
     const uint32_t sw = (r16 >> 1) & 7u;
     const uint32_t fra = (wm * (16u * MT) + r16) * 128u, frb = BM * 128u + (wn * (16u * NT) + r16) * 128u;
-    auto multiply = [&](uint32_t slot, uint32_t step) __attribute__((always_inline)) {
-        const int8_t* const A = lds + slot * STAGE + fra;
-        const int8_t* const B = lds + slot * STAGE + frb;
+    // a half of a step (64 bytes of every row) into fragments
+    auto frags = [&](uint32_t slot, uint32_t h, v4i (&xa)[MT], v4i (&xb)[NT]) __attribute__((always_inline)) {
+        const int8_t* const S = lds + slot * STAGE;
+        const uint32_t c = ((h * 4u + q) ^ sw) * 16u;
 #pragma unroll
+        for (int j = 0; j < NT; ++j) xb[j] = *reinterpret_cast<const v4i*>(S + frb + j * 2048 + c);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xa[i] = *reinterpret_cast<const v4i*>(S + fra + i * 2048 + c);
+    };
+    auto mfma_row = [&](int i, const v4i (&xa)[MT], const v4i (&xb)[NT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+    };
+    auto multiply_last = [&](uint32_t slot, uint32_t step) __attribute__((always_inline)) {   // a step that is not whole
+#pragma unroll 1
         for (uint32_t h = 0; h < 2u; ++h) {
             const uint32_t k = step * 128u + h * 64u;
             if (k >= p.dim) break;
-            const uint32_t c = ((h * 4u + q) ^ sw) * 16u;
             v4i xa[MT], xb[NT];
+            frags(slot, h, xa, xb);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) xb[j] = *reinterpret_cast<const v4i*>(B + j * 2048 + c);
+            for (int i = 0; i < MT; ++i) xa[i] = mask_chunk(xa[i], k + q * 16u, p.dim);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xa[i] = *reinterpret_cast<const v4i*>(A + i * 2048 + c);
-            if (k + 64u > p.dim) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i) xa[i] = mask_chunk(xa[i], k + q * 16u, p.dim);
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+            for (int i = 0; i < MT; ++i) mfma_row(i, xa, xb);
         }
     };
+    // The loop meets once a step, in its middle: the second half's fragments are read while the first half multiplies; then the
+    // waves meet -- this step's stage has been read, the next one's has landed --, and while the second half multiplies the
+    // stage is filled again and the next step's first fragments are read. The matrix cores wait for neither.
+    const uint32_t whole = min(steps, p.dim / 128u - min(first, p.dim / 128u));   // steps without an end of the rows
+    v4i fa0[MT], fb0[NT], fa1[MT], fb1[NT];
     if constexpr (DMA) {
 #pragma unroll
-        for (uint32_t s = 0; s < ST - 1u; ++s)
+        for (uint32_t s = 0; s < (uint32_t)ST; ++s)
             if (s < steps) transfer(s, first + s);
-        uint32_t slot = 0;
-        for (uint32_t s = 0; s < rounds; ++s) {
-            // (in flight behind this step's: those of the next ST - 2, if there are as many)
-            if (ST > 2 && s + (ST - 1u) <= steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (PA + PB)) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (s + (ST - 1u) < steps) transfer(slot == 0 ? ST - 1u : slot - 1u, first + s + (ST - 1u));
-            if (KG == 1 || s < steps) multiply(slot, first + s);
-            slot = slot + 1u == ST ? 0u : slot + 1u;
-        }
+        if (ST <= (int)steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * (PA + PB)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     } else {
-        if (KG == 1 || steps) {
-            transfer(0, first);
-            put(0);
-        }
-        for (uint32_t s = 0; s < rounds; ++s) {
+        if (steps > 0) { transfer(0, first); put(0); }
+        if (AHEAD && steps > 1) { transfer(1, first + 1u); put(1); }
+        if (AHEAD && steps > 2) transfer(0, first + 2u);
+    }
+    __syncthreads();
+    uint32_t slot = 0, s = 0;
+    if constexpr (!AHEAD) {
+        for (; s < whole; ++s) {   // (the next step's loads are in flight while this one multiplies)
+            if (s + 1u < steps) transfer(0, first + s + 1u);
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h) {
+                frags(slot, h, fa0, fb0);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) mfma_row(i, fa0, fb0);
+            }
+            slot ^= 1u;
+            if (s + 1u < steps) put(slot);
             __syncthreads();
-            if (s + 1u < steps) transfer((s + 1u) & 1u, first + s + 1u);
-            if (KG == 1 || s < steps) multiply(s & 1u, first + s);
-            if (s + 1u < steps) put((s + 1u) & 1u);
         }
     }
+    if constexpr (AHEAD) frags(0, 0, fa0, fb0);
+    for (; AHEAD && s < whole; ++s) {
+        const uint32_t next = slot + 1u == (uint32_t)ST ? 0u : slot + 1u;
+        frags(slot, 1, fa1, fb1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) mfma_row(i, fa0, fb0);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (DMA) {   // the next step's transfers are in; those of up to ST - 2 more may be on their way
+            if (ST == 2 || s + (uint32_t)ST <= steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * (PA + PB)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __syncthreads();
+        if constexpr (!DMA)
+            if (s + 2u < steps) put(slot);
+        frags(next, 0, fa0, fb0);   // (behind the last step: of no use, of no harm)
+        __builtin_amdgcn_sched_barrier(0);
+        // (a transfer behind every few multiplications; two, four or all of them together take the same time)
+        const bool more = s + (uint32_t)ST < whole;
+        if constexpr (DMA) {
+            if (!more && s + (uint32_t)ST < steps) transfer(slot, first + s + (uint32_t)ST);
+        } else {
+            if (s + 3u < steps) transfer(0, first + s + 3u);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if constexpr (DMA) {
+                if (more) {
+#pragma unroll
+                    for (int x = 0; x < PA + PB; ++x)
+                        if (x * MT / (PA + PB) == i) piece(slot, first + s + (uint32_t)ST, x);
+                }
+            }
+            mfma_row(i, fa1, fb1);
+            if constexpr (DMA) __builtin_amdgcn_sched_barrier(0);
+        }
+        slot = next;
+    }
+    if (whole < steps) multiply_last(slot, first + whole);
+    for (; s < rounds; ++s) __syncthreads();   // (a group with fewer steps passes the others' meetings)
     __syncthreads();
     // the groups' sums joined two by two: half of those left hand theirs over, half add
     if constexpr (KG > 1) {
@@ -353,7 +418,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
     }
     // 16 rows of the wave's columns at a time through a piece of LDS of its own: a store then covers whole runs of a row
     E* const out = reinterpret_cast<E*>(p.out);
-    E* const piece = reinterpret_cast<E*>(all) + wid * (16u * LDO);
+    E* const block = reinterpret_cast<E*>(all) + wid * (16u * LDO);
     float sb[NT];
     const uint32_t col0 = n0 + wn * RUN;
 #pragma unroll
@@ -370,7 +435,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
             const uint32_t row = row0 + q * 4u + (uint32_t)r;
             const float sa = p.sa && row < p.m ? p.sa[row] : 1.0f;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) *(piece + (q * 4u + (uint32_t)r) * LDO + (uint32_t)j * 16u + r16) = T::round(scaled(acc[i][j][r], sa, sb[j]));
+            for (int j = 0; j < NT; ++j) *(block + (q * 4u + (uint32_t)r) * LDO + (uint32_t)j * 16u + r16) = T::round(scaled(acc[i][j][r], sa, sb[j]));
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -381,7 +446,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG) mm_tile_kernel(const MmArgs
         for (uint32_t r = 0; r < 16u; r += RPI) {
             const uint32_t lr = r + lane / LPR, row = row0 + lr, c = (lane % LPR) * PER;
             if (lr < 16u && row < p.m) {
-                const E* const from = piece + lr * LDO + c;
+                const E* const from = block + lr * LDO + c;
                 E* const to = out + (uint64_t)row * p.ldo + col0 + c;
                 if (col0 + c + PER <= p.n) *reinterpret_cast<evec*>(to) = *reinterpret_cast<const evec*>(from);
                 else
@@ -416,18 +481,18 @@ bool dma_fits(const MmArgs& p) {
 }
 
 // Which tile. Every form gives the same bits, so the choice is one of time alone: the one with the least
-//   2.5 us + max(rounds (fix + per * steps a group of waves does), bytes the tiles read / rate + output / 5 TB/s),
+//   max(rounds (fix + per * steps a group of waves does), operands and output / 5.3 TB/s + what tiles read again / 14 TB/s),
 // rounds = tiles over what 256 CUs hold at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
-// up. The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
+// up (11 TB/s for rows at any byte). The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
 //   16 x 4096 x 4096   16 x 64 tiles in 4 groups   7.2    in 1   14.7 (n 16384)   32 x 64 in 4   8.2
-//   64 x 4096 x 4096   32 x 64 in 4   8.8    64 x 64 in 2  10.9    in 1  15.6
-//   256 x 4096 x 4096  64 x 64 in 2  11.6    128 x 128 in 2  21.7    in 1  33.1    256 x 256  50
-//   1024 x 4096 x 4096 128 x 128 in 2  23.7    64 x 64 in 1  29.5    128 x 128 in 1  34.4    256 x 256  51
-//   4096 x 16384 x 4096  256 x 256  239    128 x 128 in 1  355
-//   1 x 1M x 384  16 x 64 in 1  69    64 x 1M x 384  64 x 128  114, 64 x 64  127    128 x 1M x 384  128 x 128  179, 64 x 64  235
+//   64 x 4096 x 4096   32 x 64 in 4   8.7    64 x 64 in 2  10.4    in 1  18.4
+//   256 x 4096 x 4096  64 x 64 in 2  11.3    in 1  19.3    128 x 128 in 2  22.2    in 1  25.8
+//   1024 x 4096 x 4096 128 x 128 in 2  25.2    64 x 128  26.8    64 x 64 in 1  27.4    128 x 128 in 1  27.7    256 x 256  47
+//   4096 x 16384 x 4096  256 x 256  242    128 x 128 in 1  303
+//   1 x 1M x 384  16 x 64 in 1  66    64 x 1M x 384  64 x 128  112, 64 x 64  126    128 x 1M x 384  128 x 128  178, 64 x 64  235
 // and for rows at any byte (through registers):
-//   30 x 50021 x 777  32 x 64  12.6, 64 x 64  13.4    512 x 4096 x 4001  64 x 64  27.8, 64 x 128  33.0
-//   1024 x 4096 x 4001  64 x 128  36.9, 128 x 128  42.6    4096 x 8192 x 4001  256 x 256  157, 128 x 128  223
+//   30 x 50021 x 777  32 x 64  12.6, 64 x 64  13.4    512 x 4096 x 4001  64 x 64  22.9, 64 x 128  23.7, 128 x 128  30.2
+//   1024 x 4096 x 4001  128 x 128  31.6, 64 x 128  33.9, 64 x 64  43.5    4096 x 8192 x 4001  256 x 256  157, 128 x 128  206
 enum TileForm { T16, T16G4, T32, T32G4, T64, T64G2, T64G4, T64x128, T128, T128G2, T256, N_FORMS };
 struct FormCost {
     uint16_t bm, bn, groups, threads;
@@ -436,18 +501,19 @@ struct FormCost {
 };
 constexpr FormCost DMA_COST[N_FORMS] = {
     {16, 64, 1, 128, 5, 4.0f, 0.30f, 0.38f},   {16, 64, 4, 512, 1, 2.5f, 0.28f, 0.30f}, {32, 64, 1, 128, 6, 5.5f, 0.45f, 0.50f},
-    {32, 64, 4, 512, 1, 2.2f, 0.50f, 0.55f},   {64, 64, 1, 256, 5, 3.5f, 0.36f, 0.73f}, {64, 64, 2, 512, 1, 2.3f, 0.42f, 0.43f},
-    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.5f, 0.55f, 1.0f}, {128, 128, 1, 256, 2, 5.0f, 0.60f, 1.25f},
-    {128, 128, 2, 512, 1, 6.5f, 0.85f, 0.92f}, {256, 256, 1, 512, 1, 8.5f, 1.30f, 1.60f}};
+    {32, 64, 4, 512, 1, 2.2f, 0.50f, 0.55f},   {64, 64, 1, 256, 5, 3.5f, 0.36f, 0.70f}, {64, 64, 2, 512, 1, 2.3f, 0.40f, 0.42f},
+    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.5f, 0.45f, 0.76f}, {128, 128, 1, 256, 2, 5.0f, 0.50f, 0.95f},
+    {128, 128, 2, 512, 1, 6.5f, 0.85f, 0.98f}, {256, 256, 1, 512, 1, 8.5f, 1.30f, 1.60f}};
 constexpr FormCost ANY_COST[N_FORMS] = {
     {16, 64, 1, 128, 8, 3.0f, 0.43f, 0.60f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},   {32, 64, 1, 128, 6, 3.0f, 0.48f, 0.80f},
-    {32, 64, 4, 512, 1, 2.5f, 1.05f, 1.15f},   {64, 64, 1, 256, 5, 2.0f, 0.58f, 1.60f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
-    {64, 64, 4, 1024, 1, 2.0f, 1.50f, 1.60f},  {64, 128, 1, 256, 3, 3.0f, 0.80f, 1.45f}, {128, 128, 1, 256, 2, 4.0f, 0.90f, 1.60f},
+    {32, 64, 4, 512, 1, 2.5f, 1.05f, 1.15f},   {64, 64, 1, 256, 5, 2.0f, 0.30f, 1.40f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
+    {64, 64, 4, 1024, 1, 2.0f, 1.30f, 1.45f},  {64, 128, 1, 256, 3, 3.0f, 0.30f, 1.27f}, {128, 128, 1, 256, 2, 4.0f, 0.50f, 1.42f},
     {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},   {256, 256, 1, 512, 1, 7.0f, 1.80f, 2.20f}};
 
 int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
     constexpr double CUS = 256.0;
     const double steps = (double)((p.dim + 127u) / 128u);
+    const double once = ((double)p.m + (double)p.n) * p.dim;
     int best = T256;
     double least = 1e300;
     for (int f = 0; f < N_FORMS; ++f) {
@@ -458,7 +524,8 @@ int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
         const double at_once = CUS * c.held, full = tiles < at_once ? tiles / at_once : 1.0;
         const double rounds = __builtin_ceil(tiles / at_once);
         const double busy = rounds * (c.fix + (c.lo + (c.hi - c.lo) * full) * __builtin_ceil(steps / c.groups));
-        const double moved = tiles * (c.bm + c.bn) * (double)p.dim / (dma ? 8.0e6 : 6.5e6) + (double)p.m * p.n * out_bytes / 5.0e6;
+        const double again = tiles * (c.bm + c.bn) * (double)p.dim - once;
+        const double moved = (once + (double)p.m * p.n * out_bytes) / 5.3e6 + (again > 0.0 ? again : 0.0) / (dma ? 14.0e6 : 11.0e6);
         const double t = busy > moved ? busy : moved;
         if (t < least) {
             least = t;
