@@ -374,10 +374,25 @@ def test_store_rows_as_8_bits(trag):
             x = torch.from_numpy(rows[row0:row0 + n]).cuda()
             _check_rows(x, None, None, 0.0, q8[:, :d], scale, norm=False)
         assert (q8[:, d:] == FILL).all()
+    # a row that is replaced while its quantisation still waits on a busy stream: the call has the row it was given
+    busy = torch.randn((8192, 8192), device="cuda")
+    q8 = torch.empty((5000, d), dtype=torch.int8, device="cuda")
+    scale = torch.empty(5000, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            busy @ busy
+    store.quantize_device(0, 5000, q8.data_ptr(), d, scale.data_ptr(), side.cuda_stream)
+    trag._abi.check(trag.lib().trag_store_overwrite(store.handle, 17, (100 * rows[17]).ctypes.data_as(trag._abi._fp), d))
+    torch.cuda.synchronize()
+    _check_rows(torch.from_numpy(rows).cuda(), None, None, 0.0, q8, scale, norm=False)
+    trag._abi.check(trag.lib().trag_store_overwrite(store.handle, 17, rows[17].ctypes.data_as(trag._abi._fp), d))
     with pytest.raises(trag.TragError, match="out of bounds"):
         store.quantize_device(4999, 2, q8.data_ptr(), d, scale.data_ptr())
     with pytest.raises(trag.TragError, match="stride"):
         store.quantize_device(0, 1, q8.data_ptr(), d - 1, scale.data_ptr())
+    with pytest.raises(trag.TragError, match="not device memory"):
+        store.quantize_device(0, 1, rows.ctypes.data, d, scale.data_ptr())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         with pytest.raises(trag.TragError, match="capture"):

@@ -70,7 +70,7 @@ def _loss(**kw):
 @pytest.mark.parametrize("change,words", [
     (dict(dtype=3), "element type"), (dict(n_cols=0), "0 columns"), (dict(logits_ptr=0), "null"), (dict(ids_ptr=0), "null"), (dict(teacher_ptr=0), "null"),
     (dict(loss_ptr=0), "null"), (dict(norm_ptr=0), "null"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
-    (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(logits_stride=99), "stride"),
+    (dict(temperature=float("nan")), "temperature"), (dict(temperature=1e-40), "temperature"), (dict(temperature=float("inf")), "temperature"), (dict(logits_stride=99), "stride"),
     (dict(grad_stride=99), "stride"), (dict(grad_ptr=P, grad_stride=101), "in place"), (dict(logits_ptr=P + 2), "aligned"), (dict(ids_ptr=P + 2), "aligned"),
     (dict(norm_ptr=P + 1), "aligned"), (dict(grad_ptr=P + 2), "aligned"), (dict(n_cols=80000, logits_stride=80000, grad_stride=80000), "workspace"),
     (dict(n_cols=80000, logits_stride=80000, grad_stride=80000, work_ptr=P, work_bytes=8), "workspace")])

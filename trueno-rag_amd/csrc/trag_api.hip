@@ -17,6 +17,7 @@
 
 #include "trag.h"
 #include "trag_internal.h"
+#include "trag_ops.h"
 
 using namespace trag;
 
@@ -1332,6 +1333,8 @@ trag_status trag_store_overwrite(trag_store* s, uint32_t row, const float* vec, 
     if (row >= s->n_rows) return fail(TRAG_INVALID_ARG, "row out of range");
     if ((s->h_dead[row >> 5] >> (row & 31)) & 1u) return fail(TRAG_INVALID_ARG, "row was removed");
     DeviceGuard guard(s->device);
+    trag_status to = order_after_last(s, s->stream);   // (what the handle enqueued on a caller's stream may still be reading the row)
+    if (to != TRAG_OK) return to;
     float* dst = s->d_rows + (size_t)row * dim;
     HIP_TRY(hipMemcpyAsync(dst, vec, (size_t)dim * sizeof(float), hipMemcpyHostToDevice, s->stream));
     HIP_TRY(launch_update_vmax(dst, 1, dim, s->d_vmax_sq, s->d_norm2 + row, s->stream));
@@ -1492,23 +1495,28 @@ trag_status trag_store_read_rows(const trag_store* s, uint64_t row0, uint64_t n,
 
 trag_status trag_store_quantize_device(trag_store* s, uint64_t row0, uint32_t n, int8_t* d_q8, uint64_t q8_stride,
                                        float* d_scale, void* hip_stream) {
-    if (!s) return fail(TRAG_INVALID_ARG, "null store");
-    std::lock_guard<std::mutex> lk(s->mu);
-    if (row0 + n > s->n_rows || row0 + n < row0) return fail(TRAG_INVALID_ARG, "row range out of bounds");
-    if (n == 0) return TRAG_OK;
-    if (!d_q8 || !d_scale) return fail(TRAG_INVALID_ARG, "null argument");
-    if (q8_stride < s->cfg.dim) return fail(TRAG_INVALID_ARG, "a row stride is less than the dimension");
-    DeviceGuard guard(s->device);
-    hipStream_t st = (hipStream_t)hip_stream;
-    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (st && hipStreamIsCapturing(st, &cap) != hipSuccess) { (void)hipGetLastError(); cap = hipStreamCaptureStatusNone; }
-    if (cap != hipStreamCaptureStatusNone)
-        return fail(TRAG_UNSUPPORTED, "a store's rows move when it grows: not for stream capture");
-    trag_status ts = order_after_last(s, st);   // (behind the copies of small inserts on the store's stream)
-    if (ts != TRAG_OK) return ts;
-    HIP_TRY(launch_quantize_rows_f32(s->d_rows + (size_t)row0 * s->cfg.dim, s->cfg.dim, n, s->cfg.dim, d_q8, q8_stride,
-                                     d_scale, st));
-    return TRAG_OK;
+    return op_entry([&]() -> trag_status {
+        if (!s) return fail(TRAG_INVALID_ARG, "null store");
+        std::lock_guard<std::mutex> lk(s->mu);
+        if (row0 + n > s->n_rows || row0 + n < row0) return fail(TRAG_INVALID_ARG, "row range out of bounds");
+        if (n == 0) return TRAG_OK;
+        if (!d_q8 || !d_scale) return fail(TRAG_INVALID_ARG, "null argument");
+        if (q8_stride < s->cfg.dim) return fail(TRAG_INVALID_ARG, "a row stride is less than the dimension");
+        if (!aligned_to(d_scale, 4)) return fail(TRAG_INVALID_ARG, "an array is not aligned to its elements");
+        DeviceGuard guard(s->device);
+        OpDevice on("trag_store_quantize_device", hip_stream, {s->d_rows, d_q8, d_scale});
+        if (on.status != TRAG_OK) return on.status;
+        hipStream_t st = (hipStream_t)hip_stream;
+        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+        if (st && hipStreamIsCapturing(st, &cap) != hipSuccess) { (void)hipGetLastError(); cap = hipStreamCaptureStatusNone; }
+        if (cap != hipStreamCaptureStatusNone)
+            return fail(TRAG_UNSUPPORTED, "a store's rows move when it grows: not for stream capture");
+        trag_status ts = order_after_last(s, st);   // (behind the copies of small inserts on the store's stream)
+        if (ts != TRAG_OK) return ts;
+        HIP_TRY(launch_quantize_rows_f32(s->d_rows + (size_t)row0 * s->cfg.dim, s->cfg.dim, n, s->cfg.dim, d_q8, q8_stride,
+                                         d_scale, st));
+        return TRAG_OK;
+    });
 }
 
 trag_status trag_store_search_device(trag_store* s, const float* d_queries, uint32_t n_queries,
