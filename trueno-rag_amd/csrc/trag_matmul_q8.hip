@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(64 * WK * WN) mm_direct_kernel(const MmArgs p)
 // way; the permutation is applied to the addresses that the lanes fetch), ST stages deep. Otherwise the same through
 // registers, two stages.
 // KG: groups of waves that share a tile's terms, each with stages of its own, where there are few tiles.
-// What bounds it (4096 x 16384 x 4096, 242 us, 2.27 POP/s; 8192 x 8192 x 8192 442 us, 2.49): the matrix cores at the 2.0 GHz
+// What bounds it (4096 x 16384 x 4096, 236 us, 2.33 POP/s; 8192 x 8192 x 8192 440 us, 2.50): the matrix cores at the 2.0 GHz
 // that they hold under this load are half busy, fragment reads 22 % of LDS's cycles; reading fragments ahead of the
 // multiplications (128 x 128 tiles 355 -> 303 us) and moving the transfers within a step do not change the largest tile's time.
 // A plain large 8-bit library product takes 288 and 527 us for the two.
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mm_tile_kernel(const MmA
     };
     auto mfma_row = [&](int i, const v4i (&xa)[MT], const v4i (&xb)[NT]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xa[i], xb[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(xb[j], xa[i], acc[i][j], 0, 0, 0);
     };
     auto multiply_last = [&](uint32_t slot, uint32_t step) __attribute__((always_inline)) {   // a step that is not whole
 #pragma unroll 1
@@ -416,47 +416,64 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mm_tile_kernel(const MmA
         }
         if (kg > 0) return;
     }
-    // 16 rows of the wave's columns at a time through a piece of LDS of its own: a store then covers whole runs of a row
+    // b's rows came first in the multiplications: lane l holds row l % 16 and columns 4 (l / 16) .. + 3 of every 16 x 16 block,
+    // which go side by side into a piece of LDS of the wave's own, 16 rows at a time; read back along the rows, a store
+    // covers whole runs of a row. (A wave's LDS accesses are served in order.)
     E* const out = reinterpret_cast<E*>(p.out);
     E* const block = reinterpret_cast<E*>(all) + wid * (16u * LDO);
-    float sb[NT];
-    const uint32_t col0 = n0 + wn * RUN;
+    typedef E evec __attribute__((ext_vector_type(16 / sizeof(E)), aligned(sizeof(E))));
+    typedef E four __attribute__((ext_vector_type(4)));
+    typedef float scale4 __attribute__((ext_vector_type(4), aligned(4)));
+    const uint32_t col0 = n0 + wn * RUN, row00 = m0 + wm * (16u * MT);
+    scale4 sb[NT];
+    float sa[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const uint32_t col = col0 + (uint32_t)j * 16u + r16;
-        sb[j] = p.sb && col < p.n ? p.sb[col] : 1.0f;
+        const uint32_t col = col0 + (uint32_t)j * 16u + q * 4u;
+        sb[j] = scale4{1.0f, 1.0f, 1.0f, 1.0f};
+        if (p.sb) {
+            if (col + 4u <= p.n) sb[j] = *reinterpret_cast<const scale4*>(p.sb + col);
+            else
+#pragma unroll
+                for (uint32_t r = 0; r < 4u; ++r)
+                    if (col + r < p.n) sb[j][r] = p.sb[col + r];
+        }
     }
-    typedef E evec __attribute__((ext_vector_type(16 / sizeof(E)), aligned(sizeof(E))));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = p.sa ? p.sa[min(row00 + (uint32_t)i * 16u + r16, p.m - 1u)] : 1.0f;
+    constexpr uint32_t LPR = RUN / PER;                           // lanes a row
+    constexpr uint32_t RPI = 64u / LPR < 16u ? 64u / LPR : 16u;   // rows a wave-instruction
+    const uint32_t c = (lane % LPR) * PER;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const uint32_t row0 = m0 + wm * (16u * MT) + (uint32_t)i * 16u;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t row = row0 + q * 4u + (uint32_t)r;
-            const float sa = p.sa && row < p.m ? p.sa[row] : 1.0f;
+        for (int j = 0; j < NT; ++j) {
+            four v;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) *(block + (q * 4u + (uint32_t)r) * LDO + (uint32_t)j * 16u + r16) = T::round(scaled(acc[i][j][r], sa, sb[j]));
+            for (int r = 0; r < 4; ++r) v[r] = T::round(scaled(acc[i][j][r], sa[i], sb[j][r]));
+            *reinterpret_cast<four*>(block + r16 * LDO + (uint32_t)j * 16u + q * 4u) = v;
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        constexpr uint32_t LPR = RUN / PER;                // lanes a row
-        constexpr uint32_t RPI = 64u / LPR < 16u ? 64u / LPR : 16u;   // rows a wave-instruction
+        evec v[16u / RPI];
 #pragma unroll
-        for (uint32_t r = 0; r < 16u; r += RPI) {
-            const uint32_t lr = r + lane / LPR, row = row0 + lr, c = (lane % LPR) * PER;
+        for (uint32_t r = 0; r < 16u / RPI; ++r) v[r] = *reinterpret_cast<const evec*>(block + min(r * RPI + lane / LPR, 15u) * LDO + c);
+#pragma unroll
+        for (uint32_t r = 0; r < 16u / RPI; ++r) {
+            const uint32_t lr = r * RPI + lane / LPR, row = row00 + (uint32_t)i * 16u + lr;
             if (lr < 16u && row < p.m) {
-                const E* const from = block + lr * LDO + c;
                 E* const to = out + (uint64_t)row * p.ldo + col0 + c;
-                if (col0 + c + PER <= p.n) *reinterpret_cast<evec*>(to) = *reinterpret_cast<const evec*>(from);
+                if (col0 + c + PER <= p.n) *reinterpret_cast<evec*>(to) = v[r];
                 else
+#pragma unroll
                     for (uint32_t x = 0; x < PER; ++x)
-                        if (col0 + c + x < p.n) to[x] = from[x];
+                        if (col0 + c + x < p.n) to[x] = v[r][x];
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
 
@@ -481,18 +498,18 @@ bool dma_fits(const MmArgs& p) {
 }
 
 // Which tile. Every form gives the same bits, so the choice is one of time alone: the one with the least
-//   max(rounds (fix + per * steps a group of waves does), operands and output / 5.3 TB/s + what tiles read again / 14 TB/s),
+//   max(rounds (fix + per * steps a group of waves does), operands and output / 6 TB/s + what tiles read again / 16 TB/s),
 // rounds = tiles over what 256 CUs hold at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
-// up (11 TB/s for rows at any byte). The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
-//   16 x 4096 x 4096   16 x 64 tiles in 4 groups   7.2    in 1   14.7 (n 16384)   32 x 64 in 4   8.2
-//   64 x 4096 x 4096   32 x 64 in 4   8.7    64 x 64 in 2  10.4    in 1  18.4
-//   256 x 4096 x 4096  64 x 64 in 2  11.3    in 1  19.3    128 x 128 in 2  22.2    in 1  25.8
-//   1024 x 4096 x 4096 128 x 128 in 2  25.2    64 x 128  26.8    64 x 64 in 1  27.4    128 x 128 in 1  27.7    256 x 256  47
-//   4096 x 16384 x 4096  256 x 256  242    128 x 128 in 1  303
-//   1 x 1M x 384  16 x 64 in 1  66    64 x 1M x 384  64 x 128  112, 64 x 64  126    128 x 1M x 384  128 x 128  178, 64 x 64  235
+// up (12 TB/s for rows at any byte). The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
+//   16 x 4096 x 4096   16 x 64 tiles in 4 groups of waves  7.2    in 1  16.3    32 x 64 in 4   7.7
+//   64 x 4096 x 4096   32 x 64 in 4   8.0    64 x 64 in 2   9.7    in 1  17.5
+//   256 x 4096 x 4096  64 x 64 in 2  10.3    in 1  18.0    128 x 128 in 2  20.1    in 1  24.0
+//   1024 x 4096 x 4096 128 x 128 in 2  22.7    64 x 128  25.0    128 x 128 in 1  25.9    64 x 64 in 1  28.7    256 x 256  44.5
+//   4096 x 16384 x 4096  256 x 256  235    128 x 128 in 1  290
+//   1 x 1M x 384  16 x 64 in 1  66    64 x 1M x 384  64 x 128  102, 64 x 64  108    128 x 1M x 384  128 x 128  136, 64 x 64  180
 // and for rows at any byte (through registers):
-//   30 x 50021 x 777  32 x 64  12.6, 64 x 64  13.4    512 x 4096 x 4001  64 x 64  22.9, 64 x 128  23.7, 128 x 128  30.2
-//   1024 x 4096 x 4001  128 x 128  31.6, 64 x 128  33.9, 64 x 64  43.5    4096 x 8192 x 4001  256 x 256  157, 128 x 128  206
+//   37 x 50021 x 777  64 x 128  12.2, 64 x 64  13.5    512 x 4096 x 4001  64 x 64  22.6, 64 x 128  23.0, 128 x 128  28.8
+//   1024 x 4096 x 4001  128 x 128  29.9, 64 x 128  33.1, 64 x 64  42.1    4096 x 8192 x 4001  256 x 256  150, 128 x 128  189
 enum TileForm { T16, T16G4, T32, T32G4, T64, T64G2, T64G4, T64x128, T128, T128G2, T256, N_FORMS };
 struct FormCost {
     uint16_t bm, bn, groups, threads;
@@ -500,15 +517,15 @@ struct FormCost {
     float fix, lo, hi;
 };
 constexpr FormCost DMA_COST[N_FORMS] = {
-    {16, 64, 1, 128, 5, 4.0f, 0.30f, 0.38f},   {16, 64, 4, 512, 1, 2.5f, 0.28f, 0.30f}, {32, 64, 1, 128, 6, 5.5f, 0.45f, 0.50f},
-    {32, 64, 4, 512, 1, 2.2f, 0.50f, 0.55f},   {64, 64, 1, 256, 5, 3.5f, 0.36f, 0.70f}, {64, 64, 2, 512, 1, 2.3f, 0.40f, 0.42f},
-    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.5f, 0.45f, 0.76f}, {128, 128, 1, 256, 2, 5.0f, 0.50f, 0.95f},
-    {128, 128, 2, 512, 1, 6.5f, 0.85f, 0.98f}, {256, 256, 1, 512, 1, 8.5f, 1.30f, 1.60f}};
+    {16, 64, 1, 128, 5, 3.7f, 0.30f, 0.38f},   {16, 64, 4, 512, 1, 2.4f, 0.28f, 0.30f}, {32, 64, 1, 128, 6, 5.0f, 0.45f, 0.50f},
+    {32, 64, 4, 512, 1, 1.9f, 0.48f, 0.52f},   {64, 64, 1, 256, 5, 3.0f, 0.36f, 0.70f}, {64, 64, 2, 512, 1, 1.8f, 0.38f, 0.40f},
+    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.0f, 0.45f, 0.76f}, {128, 128, 1, 256, 2, 3.8f, 0.50f, 0.90f},
+    {128, 128, 2, 512, 1, 4.6f, 0.85f, 0.98f}, {256, 256, 1, 512, 1, 7.5f, 1.30f, 1.60f}};
 constexpr FormCost ANY_COST[N_FORMS] = {
-    {16, 64, 1, 128, 8, 3.0f, 0.43f, 0.60f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},   {32, 64, 1, 128, 6, 3.0f, 0.48f, 0.80f},
-    {32, 64, 4, 512, 1, 2.5f, 1.05f, 1.15f},   {64, 64, 1, 256, 5, 2.0f, 0.30f, 1.40f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
-    {64, 64, 4, 1024, 1, 2.0f, 1.30f, 1.45f},  {64, 128, 1, 256, 3, 3.0f, 0.30f, 1.27f}, {128, 128, 1, 256, 2, 4.0f, 0.50f, 1.42f},
-    {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},   {256, 256, 1, 512, 1, 7.0f, 1.80f, 2.20f}};
+    {16, 64, 1, 128, 8, 2.7f, 0.43f, 0.60f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},   {32, 64, 1, 128, 6, 2.6f, 0.46f, 0.78f},
+    {32, 64, 4, 512, 1, 2.2f, 1.03f, 1.12f},   {64, 64, 1, 256, 5, 1.7f, 0.30f, 1.38f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
+    {64, 64, 4, 1024, 1, 1.6f, 1.28f, 1.43f},  {64, 128, 1, 256, 3, 2.6f, 0.30f, 1.26f}, {128, 128, 1, 256, 2, 3.2f, 0.50f, 1.36f},
+    {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},   {256, 256, 1, 512, 1, 6.0f, 1.80f, 2.20f}};
 
 int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
     constexpr double CUS = 256.0;
@@ -525,7 +542,7 @@ int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
         const double rounds = __builtin_ceil(tiles / at_once);
         const double busy = rounds * (c.fix + (c.lo + (c.hi - c.lo) * full) * __builtin_ceil(steps / c.groups));
         const double again = tiles * (c.bm + c.bn) * (double)p.dim - once;
-        const double moved = (once + (double)p.m * p.n * out_bytes) / 5.3e6 + (again > 0.0 ? again : 0.0) / (dma ? 14.0e6 : 11.0e6);
+        const double moved = (once + (double)p.m * p.n * out_bytes) / 6.0e6 + (again > 0.0 ? again : 0.0) / (dma ? 16.0e6 : 12.0e6);
         const double t = busy > moved ? busy : moved;
         if (t < least) {
             least = t;
