@@ -7,9 +7,9 @@
 //
 // The loss needs two numbers of the whole row, m = max z and ln sum exp((z - m) / T), and k logits; the
 // gradient needs the row again. Bound by HBM: one read of the logits for the loss, one read and one write
-// for a gradient. Rows of up to 32768 columns stay in registers between the sum and the gradient (as
-// exponentials, so nothing is computed twice); longer rows are cut into chunks whose partial (m, sum)
-// pairs are joined by a second launch, which also fills the chip when there are few rows.
+// for a gradient. Rows of up to 65536 columns stay in registers between the sum and the gradient; longer rows
+// are cut into chunks, each in the registers of one workgroup, whose partial (m, sum) pairs are joined by a second
+// launch, and which read the logits again for a gradient.
 //
 // Exponentials go through exp2 of (z - m) log2(e) / T: the difference first, so that rows at the type's lowest
 // value, whose product with 1 / T would overflow, still come out as the distribution they are. Sums over a
@@ -31,7 +31,10 @@ struct F32by8 {
 constexpr uint32_t LIST_MAX = 1024;        // teacher entries per row
 constexpr uint32_t ROW_MAX = 65536;        // columns of the row kernel
 constexpr uint32_t PART_STEP = 2048;       // a chunk of a long row is a multiple of this
-constexpr uint32_t PART_MAX = 8192;        // (gradient of 4096 x 32000 bf16: 111 us, with 16384 117, with 32768 124)
+// ... and at most what 256 threads hold as four vectors each (gradient of 4096 x 32000 bf16: 102 us, 5.1 TB/s; two vectors
+// 125, eight 102; reading the logits where each is needed 116)
+constexpr int PART_VECS = 4;
+constexpr uint32_t PART_MAX = 256u * 8u * PART_VECS;
 
 struct DistillArgs {
     const void* z;
@@ -271,15 +274,18 @@ __global__ void __launch_bounds__(NT, NT == 256 && sizeof(typename T::elem) == 2
         if constexpr (GRAD) l.enter(a, list, 0u, a.n_cols);
         l.sums(a, lt, ref, list);
         et = exp2_hw(expo(a, et, ref));
-        float s = et;
+        float s = et;   // (a vector's sum first: an exponential goes through at most W + NV additions in 32 bits)
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            float sv = 0.0f;
 #pragma unroll
             for (int i = 0; i < T::W; ++i) {
                 const float x = exp2_hw(expo(a, (float)h[v][i], ref));
-                s += x;
+                sv += x;
                 if constexpr (GRAD && sizeof(E) == 4) h[v][i] = x;
             }
+            s += sv;
+        }
         if constexpr (GRAD) keep_raw<T, NV>(h);
         double sum = wave_sum((double)s);
         l.sum = wave_sum(l.sum);
@@ -316,7 +322,7 @@ __global__ void __launch_bounds__(NT, NT == 256 && sizeof(typename T::elem) == 2
     }
 }
 
-// (max, sum) of one chunk of one row
+// (max, sum) of one chunk of one row; a chunk is at most PART_VECS vectors a thread
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     typedef typename T::elem E;
@@ -327,32 +333,34 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
     for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
         const uint64_t row = part / a.n_chunks;
-        const uint64_t c0 = (part % a.n_chunks) * a.chunk, c1 = min(c0 + a.chunk, (uint64_t)a.n_cols);
-        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-        float m = -INFINITY, s = 0.0f;
-        const uint64_t ct = c0 + (c1 - c0) / T::W * T::W + threadIdx.x;   // (the columns behind the last whole vector, one each)
-        if (threadIdx.x < (uint32_t)T::W && ct < c1) {
-            m = (float)z[ct];
-            s = m == m ? (m == -INFINITY ? 0.0f : (m - m == 0.0f ? 1.0f : m - m)) : m;
-            if (m != m) m = -INFINITY;
-        }
-        for (uint64_t c = c0 + threadIdx.x * T::W; c + T::W <= c1; c += NT * T::W) {
-            const typename T::vec e = load_vec<T>(z + c);
-            float top = (float)e[0];
+        const uint64_t c0 = (part % a.n_chunks) * a.chunk;
+        const uint32_t n = (uint32_t)min((uint64_t)a.chunk, a.n_cols - c0);
+        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride + c0;
+        const uint32_t whole = n / T::W * T::W, ct = whole + threadIdx.x;   // (the columns behind the last whole vector, one each)
+        typename T::vec h[PART_VECS];
+        float et = -INFINITY;
 #pragma unroll
-            for (int i = 1; i < T::W; ++i) top = fmaxf(top, (float)e[i]);
-            if (top > m) {   // (rare after the first few: the maximum of a random sequence moves ln n times)
-                s = m == -INFINITY ? s : s * exp2_hw(expo(a, m, top));
-                m = top;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int i = 0; i < T::W; ++i) s += exp2_hw(expo(a, (float)e[i], ref));
+        for (int v = 0; v < PART_VECS; ++v) {
+            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+            h[v] = fill_vec<T>(-INFINITY);
+            if (c < whole) h[v] = load_vec<T>(z + c);
         }
-        // (each wave's sum at its own maximum, then both to the workgroup's)
-        const float wm = wave_max(m), wref = wm == -INFINITY ? 0.0f : wm;
-        const double ws = wave_sum((double)s * (double)(m == -INFINITY ? 1.0f : exp2_hw(expo(a, m, wref))));
-        if (lead) { meet.top[0][wid] = wm; meet.sum[0][wid] = ws; }
+        if (threadIdx.x < (uint32_t)T::W && ct < n) et = (float)z[ct];
+        float m = et;
+#pragma unroll
+        for (int v = 0; v < PART_VECS; ++v)
+#pragma unroll
+            for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
+        // (each wave's sum at its own maximum, then the waves' at the workgroup's)
+        m = wave_max(m);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float s = exp2_hw(expo(a, et, ref));
+#pragma unroll
+        for (int v = 0; v < PART_VECS; ++v)
+#pragma unroll
+            for (int i = 0; i < T::W; ++i) s += exp2_hw(expo(a, (float)h[v][i], ref));
+        const double ws = wave_sum((double)s);
+        if (lead) { meet.top[0][wid] = m; meet.sum[0][wid] = ws; }
         __syncthreads();
         if (threadIdx.x == 0) {
             float top = meet.top[0][0];
@@ -360,7 +368,7 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
             for (int w = 1; w < NW; ++w) top = fmaxf(top, meet.top[0][w]);
             double sum = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w)
+            for (int w = 0; w < NW; ++w)   // (a wave without a number: its sum is 0, or NaN, and stays that)
                 sum += meet.sum[0][w] * (meet.top[0][w] == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, meet.top[0][w], top)));
             a.parts[2 * part] = top;
             a.parts[2 * part + 1] = (float)sum;
@@ -428,18 +436,29 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
     for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
         const uint64_t row = part / a.n_chunks;
-        const uint64_t c0 = (part % a.n_chunks) * a.chunk, c1 = min(c0 + a.chunk, (uint64_t)a.n_cols);
+        const uint32_t c0 = (uint32_t)((part % a.n_chunks) * a.chunk), c1 = c0 + min(a.chunk, a.n_cols - c0);
         const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
         E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
         Teacher<NT> l;
         l.ask(a, row);
+        const uint32_t whole = c0 + (c1 - c0) / T::W * T::W, ct = whole + threadIdx.x;
+        const bool tail = threadIdx.x < (uint32_t)T::W && ct < c1;
+        typename T::vec h[PART_VECS];
+        float et = 0.0f;
+#pragma unroll
+        for (int v = 0; v < PART_VECS; ++v) {
+            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+            h[v] = fill_vec<T>(0.0f);
+            if (c < whole - c0) h[v] = load_vec<T>(z + c0 + c);
+        }
+        if (tail) et = (float)z[ct];
         l.clear(a, list);
-        float lt = wave_max(l.template take<T>(a, row, z, (uint32_t)c0, (uint32_t)c1, list));
+        float lt = wave_max(l.template take<T>(a, row, z, c0, c1, list));
         if (lead) meet.top[1][wid] = lt;
-        __syncthreads();   // (the logits of the list have been read before any is overwritten)
+        __syncthreads();   // (everything has been read before anything is overwritten)
 #pragma unroll
         for (int w = 0; w < NW; ++w) lt = fmaxf(lt, meet.top[1][w]);
-        l.enter(a, list, (uint32_t)c0, (uint32_t)c1);
+        l.enter(a, list, c0, c1);
         l.sums(a, lt, 0.0f, list);
         l.sum = wave_sum(l.sum);
         if (lead) meet.sum[1][wid] = l.sum;
@@ -453,23 +472,26 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
         const float per_sum = (float)exp(-(double)a.norm_in[2 * row + 1]);
         const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
         const float f = gt * per_sum;
-        const uint64_t ct = c0 + (c1 - c0) / T::W * T::W + threadIdx.x;
-        if (threadIdx.x < (uint32_t)T::W && ct < c1) g[ct] = T::round(l.some ? f * exp2_hw(expo(a, (float)z[ct], ref)) : 0.0f);
-        for (uint64_t c = c0 + threadIdx.x * T::W; c + T::W <= c1; c += NT * T::W) {
-            const typename T::vec e = load_vec<T>(z + c);
+#pragma unroll
+        for (int v = 0; v < PART_VECS; ++v) {
+            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
             typename T::vec o;
 #pragma unroll
-            for (int i = 0; i < T::W; ++i) o[i] = T::round(l.some ? f * exp2_hw(expo(a, (float)e[i], ref)) : 0.0f);
-            store_vec<T>(g + c, o);
+            for (int i = 0; i < T::W; ++i) o[i] = T::round(l.some ? f * exp2_hw(expo(a, (float)h[v][i], ref)) : 0.0f);
+            if (c < whole - c0) store_vec<T>(g + c0 + c, o);
         }
+        if (tail) g[ct] = T::round(l.some ? f * exp2_hw(expo(a, et, ref)) : 0.0f);
+        // what the workgroup has written so far is in memory, in front of what follows
         __threadfence_block();
         __syncthreads();
-        if (l.some) l.template patch<T>(a, list, g, (uint32_t)c0, (uint32_t)c1, ref, per_sum, gt);
+        if (l.some) l.template patch<T>(a, list, g, c0, c1, ref, per_sum, gt);
         __syncthreads();
     }
 }
 
 uint32_t grid_of(uint64_t n) { return (uint32_t)(n < (1u << 20) ? n : (1u << 20)); }
+
+static_assert(F32by8::W == 8 && F16::W == 8 && BF16::W == 8 && PART_MAX % PART_STEP == 0, "a chunk fits the part kernels' registers");
 
 // Chunks of a long row: long ones where there are rows enough to fill the chip, short ones for few rows.
 uint32_t chunk_of(uint64_t n_rows, uint32_t n_cols) {
