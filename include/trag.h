@@ -516,7 +516,8 @@ trag_status trag_bm25_stats(trag_bm25 *ix, uint64_t *postings, uint64_t *terms);
  * TRAG_INVALID_ARG. No call allocates, synchronises, or keeps anything: all may be captured into a
  * graph and called by several threads. Strides count elements from row to row; rows may start at any
  * element (16-byte alignment is not needed, and only the product goes faster with it). A call of 0
- * rows is TRAG_OK and touches nothing. Outputs must not overlap inputs, except where said.
+ * rows is TRAG_OK and touches nothing; rows of 0 elements are TRAG_INVALID_ARG. Outputs must not overlap
+ * inputs, except where said.
  * ------------------------------------------------------------------------ */
 typedef enum trag_dtype { TRAG_F32 = 0, TRAG_F16 = 1, TRAG_BF16 = 2 } trag_dtype;
 
@@ -564,8 +565,8 @@ trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const fl
  * trag_distill_grad_device needs. d_grad NULL: the loss alone; otherwise the gradient too, in the
  * logits' type, for row weights known beforehand (d_row_weight, NULL: ones). d_grad may be d_logits
  * itself, with its stride. d_work: trag_distill_work_bytes(n_rows, n_cols) bytes, 4-byte aligned, in use
- * until the call's work is done (0 bytes, NULL, for rows of up to 65536 columns): two calls that can run at the same
- * time, two captured graphs among them, need one each. k <= 1024, else TRAG_UNSUPPORTED. */
+ * until the call's work is done (0 bytes, NULL, for rows of up to 65536 columns): two calls that can run at
+ * the same time, two captured graphs among them, need one each. k <= 1024, else TRAG_UNSUPPORTED. */
 uint64_t trag_distill_work_bytes(uint32_t n_rows, uint32_t n_cols);
 trag_status trag_distill_loss_device(const void *d_logits, uint64_t logits_stride, uint32_t dtype,
                                      uint32_t n_rows, uint32_t n_cols, const uint32_t *d_ids,

@@ -297,6 +297,78 @@ def test_product_of_rows_far_apart(trag):
             assert torch.equal(out, _expect(a, b, None, None, torch.float32))
 
 
+@pytest.mark.parametrize("m,n,dim", [(2 ** 28 + 1000, 2, 3), (2, 2 ** 28 + 1000, 16)])
+def test_product_of_very_many_rows(trag, m, n, dim):
+    """More rows than one grid of the smallest tiles covers, rows of the other operand 2^24 bytes apart where it is the wide one."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+    few, many = (n, m) if m > n else (m, n)
+    far = 2 ** 24 if m < n else dim
+    big = torch.randint(-128, 128, (many, dim), generator=g, device="cuda", dtype=torch.int8)
+    small = torch.empty(far * (few - 1) + dim, dtype=torch.int8, device="cuda").as_strided((few, dim), (far, 1))
+    small.copy_(torch.randint(-128, 128, (few, dim), generator=g, device="cuda", dtype=torch.int8))
+    scale = torch.rand(many, generator=g, device="cuda")
+    out = torch.full((m, n), float("nan"), device="cuda")
+    a, b = (big, small) if m > n else (small, big)
+    sa, sb = (scale, None) if m > n else (None, scale)
+    _product(trag, a, b, sa, sb, out, "f32")
+    for i in range(few):
+        s = torch.zeros(many, dtype=torch.int32, device="cuda")
+        for c in range(dim):
+            s += big[:, c].int() * small[i, c].int()
+        got = out[:, i] if m > n else out[i]
+        assert torch.equal(got, s.float() * scale), i
+
+
+def test_an_earlier_error_of_the_program_is_not_the_call_s(trag):
+    """A runtime call of the program that failed leaves an error behind; an operator that is launched after it succeeds."""
+    torch = _torch()
+    x = torch.ones((3, 64), device="cuda")
+    q8 = torch.empty((3, 64), dtype=torch.int8, device="cuda")
+    scale = torch.empty(3, device="cuda")
+    assert trag.lib().hipSetDevice(9999) != 0   # (the runtime that the library is linked to)
+    trag.quantize_q8_device(x.data_ptr(), 64, 0, 3, 64, q8.data_ptr(), 64, scale.data_ptr(), 0, 0, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert (q8 == 127).all()
+
+
+def test_two_threads_at_once(trag):
+    """The calls keep nothing: two threads on streams of their own, one of them the thread's default stream, get what one gets."""
+    import threading
+    torch = _torch()
+    per_thread = 2   # hipStreamPerThread
+    g = torch.Generator(device="cuda").manual_seed(4)
+    work, errors = [], []
+    for m, n, dim in ((5, 700, 384), (130, 257, 1000)):
+        x = torch.randn((m, dim), generator=g, device="cuda")
+        b = _int8(n, dim, 0, 0, g)
+        q8 = torch.zeros((m, dim), dtype=torch.int8, device="cuda")
+        work.append((x, b, q8, torch.zeros(m, device="cuda"), torch.zeros((m, n), device="cuda")))
+    streams = [torch.cuda.Stream().cuda_stream, per_thread]
+    torch.cuda.synchronize()
+
+    def run(i):
+        try:
+            x, b, q8, scale, out = work[i]
+            for _ in range(50):
+                trag.quantize_q8_device(x.data_ptr(), x.stride(0), 0, x.shape[0], x.shape[1], q8.data_ptr(), q8.stride(0), scale.data_ptr(), 0, 0, streams[i])
+                trag.matmul_q8_device(q8.data_ptr(), q8.stride(0), scale.data_ptr(), b.data_ptr(), b.stride(0), 0, x.shape[0], b.shape[0], x.shape[1], 0,
+                                      out.data_ptr(), out.stride(0), streams[i])
+        except Exception as e:   # noqa: BLE001 (handed to the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for x, b, q8, scale, out in work:
+        _check_rows(x, None, None, 0.0, q8, scale, norm=False)
+        assert torch.equal(out, _expect(q8, b, scale, None, torch.float32))
+
+
 def test_operators_on_other_streams_and_in_graphs(trag):
     """A chain norm -> product on a side stream, then captured and replayed with new inputs, with eager work
     between the replays: every replay gives what the eager chain gives."""

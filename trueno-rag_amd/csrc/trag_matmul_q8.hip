@@ -479,10 +479,25 @@ __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mm_tile_kernel(const MmA
 
 uint32_t grid8(uint64_t tiles) { return (uint32_t)((tiles + 7u) / 8u * 8u); }   // (a run of tiles for each of 8 dies)
 
+// (A grid's threads are counted in 32 bits: a product of more tiles goes out in several launches.)
 template <typename T, int MT, int NT, int WK, int WN, int U, bool SHORT = false>
 void launch_direct(const MmArgs& p, hipStream_t st) {
-    const uint64_t mt = (p.m + 16u * MT - 1u) / (16u * MT), nt = ((uint64_t)p.n + 16u * NT * WN - 1) / (16u * NT * WN);
-    hipLaunchKernelGGL((mm_direct_kernel<T, MT, NT, WK, WN, U, SHORT>), dim3(grid8(mt * nt)), dim3(64 * WK * WN), 0, st, p);
+    constexpr uint32_t BM = 16u * MT, BN = 16u * NT * WN, most = 0xFFFFFFFFu / (64u * WK * WN) - 8u;
+    const uint32_t mt = (p.m + BM - 1u) / BM, nt = (uint32_t)(((uint64_t)p.n + BN - 1u) / BN);
+    const uint32_t n_run = nt < most ? nt : most, m_run = mt < most / n_run ? mt : most / n_run;
+    for (uint32_t m0 = 0; m0 < mt; m0 += m_run)
+        for (uint32_t n0 = 0; n0 < nt; n0 += n_run) {
+            MmArgs q = p;
+            q.m = (mt - m0 <= m_run ? p.m - m0 * BM : m_run * BM);
+            q.n = (nt - n0 <= n_run ? p.n - n0 * BN : n_run * BN);
+            q.a = p.a + (uint64_t)m0 * BM * p.lda;
+            q.b = p.b + (uint64_t)n0 * BN * p.ldb;
+            if (p.sa) q.sa = p.sa + m0 * BM;
+            if (p.sb) q.sb = p.sb + n0 * BN;
+            q.out = reinterpret_cast<typename T::elem*>(p.out) + (uint64_t)m0 * BM * p.ldo + n0 * BN;
+            const uint64_t tiles = (uint64_t)((q.m + BM - 1u) / BM) * (((uint64_t)q.n + BN - 1u) / BN);
+            hipLaunchKernelGGL((mm_direct_kernel<T, MT, NT, WK, WN, U, SHORT>), dim3(grid8(tiles)), dim3(64 * WK * WN), 0, st, q);
+        }
 }
 
 template <typename T, int WM, int WN, int MT, int NT, int KG, int ST, bool DMA>

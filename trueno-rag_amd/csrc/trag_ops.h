@@ -90,6 +90,8 @@ struct OpDevice {
             }
         }
         if (dev >= 0 && hipGetDevice(&prev) == hipSuccess && prev != dev) switched = hipSetDevice(dev) == hipSuccess;
+        // (an error that a call of the program's before this one has left behind: op_launched would take it for the launch's)
+        (void)hipGetLastError();
     }
     ~OpDevice() {
         if (switched) (void)hipSetDevice(prev);
