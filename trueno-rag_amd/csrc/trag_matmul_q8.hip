@@ -512,6 +512,8 @@ bool dma_fits(const MmArgs& p) {
     return p.dim % 16u == 0 && p.lda % 16u == 0 && p.ldb % 16u == 0 && aligned_to(p.a, 16) && aligned_to(p.b, 16);
 }
 
+bool quads(const MmArgs& p) { return p.lda % 4u == 0 && p.ldb % 4u == 0 && aligned_to(p.a, 4) && aligned_to(p.b, 4); }
+
 // Which tile. Every form gives the same bits, so the choice is one of time alone: the one with the least
 //   max(rounds (fix + per * steps a group of waves does), operands and output / 6 TB/s + what tiles read again / 16 TB/s),
 // rounds = tiles over what 256 CUs hold at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
@@ -571,14 +573,14 @@ template <typename T>
 void launch_mm(const MmArgs& p, hipStream_t st) {
     if (p.dim < 16u) return launch_direct<T, 1, 8, 1, 4, 1, true>(p, st);
     // (the tiles' offsets from their first row are 32 bits, over 255 rows at most)
-    if (p.lda >= (1u << 24) || p.ldb >= (1u << 24)) return launch_direct<T, 4, 1, 8, 1, 2>(p, st);
+    if (p.lda >= (1u << 24) || p.ldb >= (1u << 24)) return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
     const bool dma = dma_fits(p);
-    // Few rows of a, short b, long rows at any byte: a wave's fragments straight from memory, eight waves a tile's terms
-    // (16 x 4096 x 4001: 7.4 us, the tiles 11.9; 30 x 2000 x 4001: 9.7, the tiles 13.5; aligned rows have the tiles ahead).
-    if (!dma && p.m <= 64u && p.n <= 8192u && p.dim >= 1024u) {
-        if (p.m <= 16u) return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
-        return launch_direct<T, 4, 1, 8, 1, 2>(p, st);
-    }
+    // Rows at any byte, few enough for a workgroup of its own on a CU for every 16 x 16 sums, and long: fragments straight from
+    // memory, eight waves a tile's terms. us, and the best of the tiles: rows at multiples of 4, 16 x 2000 x 1001 5.2, 5.6;
+    // x 3001 5.7, 7.4; x 7550 10.7, 13.2; at odd bytes 5.9, 6.3; 10.1, 11.3; 26.3, 20.9, so not those; more rows, 16 x 8000 x 3001
+    // 9.1, 9.6 and at odd bytes 16.5, 11.9. Shorter rows take the time of the launch either way.
+    if (!dma && p.dim >= 512u && (uint64_t)((p.m + 15u) / 16u) * (((uint64_t)p.n + 15u) / 16u) <= 256u && (p.dim <= 4096u || quads(p)))
+        return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
     const int form = choose_form(p, dma, sizeof(typename T::elem));
     if (dma) {
         switch (form) {
