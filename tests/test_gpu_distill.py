@@ -156,6 +156,34 @@ def test_loss_and_gradient_match_the_formula(trag, t, cols):
             assert (buf[~inside].float() == 77).all()
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1100, 1900), (1025, 4001), (2561, 25003), (2 ** 20 + 77, 5)])
+def test_many_rows(trag, t, rows, cols):
+    """The forms for many rows, and more rows than one launch takes."""
+    torch = _torch()
+    z0, ids, teacher, counts, weight = _case(rows, cols, 4, cols)
+    zb, z = _filled(z0, _types()[t], 1, 1)
+    want_loss, _, want_grad, tol_loss, _, tol_grad = _reference(z, ids, teacher, counts, 1.5, weight)
+    loss, norm, grad = torch.full((rows,), 77.0, device="cuda"), torch.full((rows, 2), 77.0, device="cuda"), torch.full_like(z, 77.0)
+    _loss(trag, t, z, ids, teacher, counts, 1.5, weight, loss, norm, grad)
+    assert ((loss.double() - want_loss).abs() <= tol_loss + 2.0 ** -149).all()
+    _check_grad(grad, want_grad, tol_grad, t)
+
+
+def test_more_chunks_than_one_launch_takes(trag):
+    torch = _torch()
+    rows, cols, k = 116_600, 65_537, 3
+    z = torch.empty((rows, cols), dtype=torch.float16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    _, ids, teacher, counts, weight = _case(rows, 1, k, 2)
+    ids = torch.randint(0, cols, (rows, k), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda", dtype=torch.int64).to(torch.int32)
+    some = torch.cat([torch.arange(20), torch.arange(rows - 200, rows, 5)]).cuda()
+    want_loss, _, want_grad, tol_loss, _, tol_grad = _reference(z[some], ids[some], teacher[some], counts[some], 2.0, weight[some])
+    loss, norm = torch.full((rows,), 77.0, device="cuda"), torch.full((rows, 2), 77.0, device="cuda")
+    _loss(trag, "f16", z, ids, teacher, counts, 2.0, weight, loss, norm, z)
+    assert ((loss[some].double() - want_loss).abs() <= tol_loss + 2.0 ** -149).all()
+    _check_grad(z[some], want_grad, tol_grad, "f16")
+
+
 def test_gradient_against_differences(trag):
     """Central differences of the 64-bit loss (step h: off by h^2 / 6 times a third derivative below 2 T, plus
     2^-52 / h times the loss), for rows with repeated ids, ids that are no column, and short lists."""

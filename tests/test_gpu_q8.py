@@ -228,6 +228,17 @@ def _expect(a, b, sa, sb, dt):
     return c.to(dt)
 
 
+def test_more_rows_than_one_launch_takes(trag):
+    torch = _torch()
+    rows = 2 ** 24 + 35
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, r = (torch.randn((rows, 3), generator=g, device="cuda") for _ in range(2))
+    q8, scale, s = torch.full((rows, 3), FILL, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros((rows, 3), device="cuda")
+    _run_norm(trag, "f32", x, r, None, 1e-6, s, q8, scale, None)
+    _check_rows(x, r, None, 1e-6, q8, scale)
+    assert torch.equal(s, x + r)
+
+
 SHAPES = [(1, 1, 1), (1, 5, 16), (1, 1000, 384), (2, 129, 15), (3, 64, 17), (7, 300, 64), (8, 257, 768), (16, 4096, 1024),
           (17, 100, 63), (31, 513, 65), (32, 64, 128), (33, 4097, 96), (64, 640, 2048), (65, 130, 129), (100, 999, 250),
           (128, 128, 64), (129, 127, 144), (200, 2000, 384), (256, 256, 512), (257, 511, 400), (300, 1030, 777), (512, 768, 1040),

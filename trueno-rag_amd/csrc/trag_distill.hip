@@ -14,6 +14,7 @@
 // Exponentials go through exp2 of (z - m) log2(e) / T: the difference first, so that rows at the type's lowest
 // value, whose product with 1 / T would overflow, still come out as the distribution they are. Sums over a
 // row are 32-bit per thread and chunk, 64-bit across them; the k terms of the loss are 64-bit.
+#include <algorithm>
 #include "trag_ops.h"
 
 namespace trag {
@@ -49,6 +50,7 @@ struct DistillArgs {
     float* parts;             // 2 per row and chunk
     uint64_t z_stride, grad_stride;
     uint32_t n_rows, n_cols, k, chunk, n_chunks;
+    uint32_t row0;            // first row of a launch
     uint32_t slot_mask;       // slots of the id table, a power of two, less one
     float temperature, c;     // c = log2(e) / T
     double c64;
@@ -229,9 +231,10 @@ __device__ __forceinline__ void keep_raw(typename T::vec (&h)[NV]) {
 
 // One workgroup a row, the row in registers as NV vectors of W columns a thread (the columns behind the last
 // whole vector: one each for the first few threads): one read of the logits, one write of the gradient, two meetings
-// of the waves and one more before the list's columns are set right.
+// of the waves and one more before the list's columns are set right. (Sixteen vectors of eight waves are held to 128 registers, so
+// that two rows fit a CU: 1000 x 50257 bf16 with the gradient 58 us, with one row a CU 71.)
 template <typename T, int NT, int NV, bool GRAD>
-__global__ void __launch_bounds__(NT, NT == 256 && sizeof(typename T::elem) == 2 && NV == 16 ? 3 : 1) distill_row_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(NT, NT == 512 && sizeof(typename T::elem) == 2 ? 4 : 1) distill_row_kernel(const DistillArgs a) {
     typedef typename T::elem E;
     constexpr int NW = NT / 64;
     __shared__ Meet<NW> meet;
@@ -240,86 +243,82 @@ __global__ void __launch_bounds__(NT, NT == 256 && sizeof(typename T::elem) == 2
     const uint32_t wid = threadIdx.x >> 6;
     const bool lead = (threadIdx.x & 63u) == 0u;
     const uint32_t whole = a.n_cols / T::W * T::W, ct = whole + threadIdx.x;
-    for (uint64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
-        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-        Teacher<NT> l;
-        l.ask(a, row);
-        // (held as they are in memory; in f32 the exponentials take their place, 16-bit types compute them again for the
-        // gradient, which costs less than the occupancy that twice the registers would)
-        // (Loads clamped to the row's last vector instead of the branches, the excess masked: 53.8 us instead of 48.6 for the
-        // loss of 4096 x 32000 bf16, no faster with the gradient.)
-        typename T::vec h[NV];
-        float et = -INFINITY;
+    const uint64_t row = (uint64_t)a.row0 + blockIdx.x;
+    const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
+    Teacher<NT> l;
+    l.ask(a, row);
+    // (held as they are in memory; in f32 the exponentials take their place, 16-bit types compute them again for the
+    // gradient, which costs less than the occupancy that twice the registers would)
+    typename T::vec h[NV];
+    float et = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+        h[v] = fill_vec<T>(-INFINITY);
+        if (c < whole) h[v] = load_vec<T>(z + c);
+    }
+    if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) et = (float)z[ct];
+    if constexpr (GRAD) l.clear(a, list);
+    float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
+    float m = et;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
+    keep_raw<T, NV>(h);
+    m = wave_max(m);
+    if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    if constexpr (GRAD) l.enter(a, list, 0u, a.n_cols);
+    l.sums(a, lt, ref, list);
+    et = exp2_hw(expo(a, et, ref));
+    float s = et;   // (a vector's sum first: an exponential goes through at most W + NV additions in 32 bits)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        float sv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < T::W; ++i) {
+            const float x = exp2_hw(expo(a, (float)h[v][i], ref));
+            sv += x;
+            if constexpr (GRAD && sizeof(E) == 4) h[v][i] = x;
+        }
+        s += sv;
+    }
+    if constexpr (GRAD) keep_raw<T, NV>(h);
+    double sum = wave_sum((double)s);
+    l.sum = wave_sum(l.sum);
+    l.cross = wave_sum(l.cross);
+    if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
+    __syncthreads();
+    sum = l.sum = l.cross = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
+    l.finish();
+    if constexpr (GRAD) {
+        E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
+        const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
+        const float f = (float)((double)gt / sum);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
-            h[v] = fill_vec<T>(-INFINITY);
-            if (c < whole) h[v] = load_vec<T>(z + c);
-        }
-        if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) et = (float)z[ct];
-        if constexpr (GRAD) l.clear(a, list);
-        float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
-        float m = et;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
-        keep_raw<T, NV>(h);
-        m = wave_max(m);
-        if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        if constexpr (GRAD) l.enter(a, list, 0u, a.n_cols);
-        l.sums(a, lt, ref, list);
-        et = exp2_hw(expo(a, et, ref));
-        float s = et;   // (a vector's sum first: an exponential goes through at most W + NV additions in 32 bits)
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float sv = 0.0f;
+            typename T::vec o;
 #pragma unroll
             for (int i = 0; i < T::W; ++i) {
-                const float x = exp2_hw(expo(a, (float)h[v][i], ref));
-                sv += x;
-                if constexpr (GRAD && sizeof(E) == 4) h[v][i] = x;
+                const float x = sizeof(E) == 4 ? (float)h[v][i] : exp2_hw(expo(a, (float)h[v][i], ref));
+                o[i] = T::round(l.some ? x * f : 0.0f);
             }
-            s += sv;
+            if (c < whole) store_vec<T>(g + c, o);
         }
-        if constexpr (GRAD) keep_raw<T, NV>(h);
-        double sum = wave_sum((double)s);
-        l.sum = wave_sum(l.sum);
-        l.cross = wave_sum(l.cross);
-        if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
+        if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) g[ct] = T::round(l.some ? et * f : 0.0f);
+        // what the workgroup has written so far is in memory, in front of what follows
+        __threadfence_block();
         __syncthreads();
-        sum = l.sum = l.cross = 0.0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
-        l.finish();
-        if constexpr (GRAD) {
-            E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
-            const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
-            const float f = (float)((double)gt / sum);
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
-                typename T::vec o;
-#pragma unroll
-                for (int i = 0; i < T::W; ++i) {
-                    const float x = sizeof(E) == 4 ? (float)h[v][i] : exp2_hw(expo(a, (float)h[v][i], ref));
-                    o[i] = T::round(l.some ? x * f : 0.0f);
-                }
-                if (c < whole) store_vec<T>(g + c, o);
-            }
-            if (threadIdx.x < (uint32_t)T::W && ct < a.n_cols) g[ct] = T::round(l.some ? et * f : 0.0f);
-            // what the workgroup has written so far is in memory, in front of what follows
-            __threadfence_block();
-            __syncthreads();
-            if (l.some) l.template patch<T>(a, list, g, 0u, a.n_cols, ref, (float)(1.0 / sum), gt);
-        }
-        if (threadIdx.x == 0) write_row(a, row, m, sum, l);
-        __syncthreads();   // (the next row uses the same arrays)
+        if (l.some) l.template patch<T>(a, list, g, 0u, a.n_cols, ref, (float)(1.0 / sum), gt);
     }
+    if (threadIdx.x == 0) write_row(a, row, m, sum, l);
 }
 
 // (max, sum) of one chunk of one row; a chunk is at most PART_VECS vectors a thread
@@ -330,50 +329,46 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     __shared__ Meet<NW> meet;
     const uint32_t wid = threadIdx.x >> 6;
     const bool lead = (threadIdx.x & 63u) == 0u;
-    const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
-    for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
-        const uint64_t row = part / a.n_chunks;
-        const uint64_t c0 = (part % a.n_chunks) * a.chunk;
-        const uint32_t n = (uint32_t)min((uint64_t)a.chunk, a.n_cols - c0);
-        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride + c0;
-        const uint32_t whole = n / T::W * T::W, ct = whole + threadIdx.x;   // (the columns behind the last whole vector, one each)
-        typename T::vec h[PART_VECS];
-        float et = -INFINITY;
+    const uint64_t part = (uint64_t)a.row0 * a.n_chunks + blockIdx.x, row = part / a.n_chunks;
+    const uint64_t c0 = (part % a.n_chunks) * a.chunk;
+    const uint32_t n = (uint32_t)min((uint64_t)a.chunk, a.n_cols - c0);
+    const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride + c0;
+    const uint32_t whole = n / T::W * T::W, ct = whole + threadIdx.x;   // (the columns behind the last whole vector, one each)
+    typename T::vec h[PART_VECS];
+    float et = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < PART_VECS; ++v) {
-            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
-            h[v] = fill_vec<T>(-INFINITY);
-            if (c < whole) h[v] = load_vec<T>(z + c);
-        }
-        if (threadIdx.x < (uint32_t)T::W && ct < n) et = (float)z[ct];
-        float m = et;
+    for (int v = 0; v < PART_VECS; ++v) {
+        const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+        h[v] = fill_vec<T>(-INFINITY);
+        if (c < whole) h[v] = load_vec<T>(z + c);
+    }
+    if (threadIdx.x < (uint32_t)T::W && ct < n) et = (float)z[ct];
+    float m = et;
 #pragma unroll
-        for (int v = 0; v < PART_VECS; ++v)
+    for (int v = 0; v < PART_VECS; ++v)
 #pragma unroll
-            for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
-        // (each wave's sum at its own maximum, then the waves' at the workgroup's)
-        m = wave_max(m);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float s = exp2_hw(expo(a, et, ref));
+        for (int i = 0; i < T::W; ++i) m = fmaxf(m, (float)h[v][i]);
+    // (each wave's sum at its own maximum, then the waves' at the workgroup's)
+    m = wave_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float s = exp2_hw(expo(a, et, ref));
 #pragma unroll
-        for (int v = 0; v < PART_VECS; ++v)
+    for (int v = 0; v < PART_VECS; ++v)
 #pragma unroll
-            for (int i = 0; i < T::W; ++i) s += exp2_hw(expo(a, (float)h[v][i], ref));
-        const double ws = wave_sum((double)s);
-        if (lead) { meet.top[0][wid] = m; meet.sum[0][wid] = ws; }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float top = meet.top[0][0];
+        for (int i = 0; i < T::W; ++i) s += exp2_hw(expo(a, (float)h[v][i], ref));
+    const double ws = wave_sum((double)s);
+    if (lead) { meet.top[0][wid] = m; meet.sum[0][wid] = ws; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float top = meet.top[0][0];
 #pragma unroll
-            for (int w = 1; w < NW; ++w) top = fmaxf(top, meet.top[0][w]);
-            double sum = 0.0;
+        for (int w = 1; w < NW; ++w) top = fmaxf(top, meet.top[0][w]);
+        double sum = 0.0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w)   // (a wave without a number: its sum is 0, or NaN, and stays that)
-                sum += meet.sum[0][w] * (meet.top[0][w] == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, meet.top[0][w], top)));
-            a.parts[2 * part] = top;
-            a.parts[2 * part + 1] = (float)sum;
-        }
-        __syncthreads();
+        for (int w = 0; w < NW; ++w)   // (a wave without a number: its sum is 0, or NaN, and stays that)
+            sum += meet.sum[0][w] * (meet.top[0][w] == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, meet.top[0][w], top)));
+        a.parts[2 * part] = top;
+        a.parts[2 * part + 1] = (float)sum;
     }
 }
 
@@ -387,40 +382,38 @@ __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
     const List list(a, lds);
     const uint32_t wid = threadIdx.x >> 6;
     const bool lead = (threadIdx.x & 63u) == 0u;
-    for (uint64_t row = blockIdx.x; row < a.n_rows; row += gridDim.x) {
-        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-        const float* const parts = a.parts + 2 * row * a.n_chunks;
-        Teacher<NT> l;
-        l.ask(a, row);
-        float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
-        // (a thread's chunks at the thread's own maximum, then to the row's)
-        float m = -INFINITY;
-        for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) m = fmaxf(m, parts[2 * c]);
-        m = wave_max(m);
-        if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
-        __syncthreads();
+    const uint64_t row = (uint64_t)a.row0 + blockIdx.x;
+    const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
+    const float* const parts = a.parts + 2 * row * a.n_chunks;
+    Teacher<NT> l;
+    l.ask(a, row);
+    float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
+    // (a thread's chunks at the thread's own maximum, then to the row's)
+    float m = -INFINITY;
+    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) m = fmaxf(m, parts[2 * c]);
+    m = wave_max(m);
+    if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
+    __syncthreads();
 #pragma unroll
-        for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
-        const float ref = m == -INFINITY ? 0.0f : m;
-        double sum = 0.0;
-        for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) {
-            const float pm = parts[2 * c];
-            // (a chunk without a number: its sum is 0, or NaN, and stays that)
-            sum += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
-        }
-        l.sums(a, lt, ref, list);
-        sum = wave_sum(sum);
-        l.sum = wave_sum(l.sum);
-        l.cross = wave_sum(l.cross);
-        if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
-        __syncthreads();
-        sum = l.sum = l.cross = 0.0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
-        l.finish();
-        if (threadIdx.x == 0) write_row(a, row, m, sum, l);
-        __syncthreads();
+    for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    double sum = 0.0;
+    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) {
+        const float pm = parts[2 * c];
+        // (a chunk without a number: its sum is 0, or NaN, and stays that)
+        sum += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
     }
+    l.sums(a, lt, ref, list);
+    sum = wave_sum(sum);
+    l.sum = wave_sum(l.sum);
+    l.cross = wave_sum(l.cross);
+    if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
+    __syncthreads();
+    sum = l.sum = l.cross = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; l.cross += meet.sum[2][w]; }
+    l.finish();
+    if (threadIdx.x == 0) write_row(a, row, m, sum, l);
 }
 
 // the gradient of one chunk of one row, from the row's saved norm
@@ -433,63 +426,68 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     const List list(a, lds);
     const uint32_t wid = threadIdx.x >> 6;
     const bool lead = (threadIdx.x & 63u) == 0u;
-    const uint64_t n_parts = (uint64_t)a.n_rows * a.n_chunks;
-    for (uint64_t part = blockIdx.x; part < n_parts; part += gridDim.x) {
-        const uint64_t row = part / a.n_chunks;
-        const uint32_t c0 = (uint32_t)((part % a.n_chunks) * a.chunk), c1 = c0 + min(a.chunk, a.n_cols - c0);
-        const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-        E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
-        Teacher<NT> l;
-        l.ask(a, row);
-        const uint32_t whole = c0 + (c1 - c0) / T::W * T::W, ct = whole + threadIdx.x;
-        const bool tail = threadIdx.x < (uint32_t)T::W && ct < c1;
-        typename T::vec h[PART_VECS];
-        float et = 0.0f;
+    const uint64_t part = (uint64_t)a.row0 * a.n_chunks + blockIdx.x, row = part / a.n_chunks;
+    const uint32_t c0 = (uint32_t)((part % a.n_chunks) * a.chunk), c1 = c0 + min(a.chunk, a.n_cols - c0);
+    const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
+    E* const g = reinterpret_cast<E*>(a.grad) + row * a.grad_stride;
+    Teacher<NT> l;
+    l.ask(a, row);
+    const uint32_t whole = c0 + (c1 - c0) / T::W * T::W, ct = whole + threadIdx.x;
+    const bool tail = threadIdx.x < (uint32_t)T::W && ct < c1;
+    typename T::vec h[PART_VECS];
+    float et = 0.0f;
 #pragma unroll
-        for (int v = 0; v < PART_VECS; ++v) {
-            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
-            h[v] = fill_vec<T>(0.0f);
-            if (c < whole - c0) h[v] = load_vec<T>(z + c0 + c);
-        }
-        if (tail) et = (float)z[ct];
-        l.clear(a, list);
-        float lt = wave_max(l.template take<T>(a, row, z, c0, c1, list));
-        if (lead) meet.top[1][wid] = lt;
-        __syncthreads();   // (everything has been read before anything is overwritten)
-#pragma unroll
-        for (int w = 0; w < NW; ++w) lt = fmaxf(lt, meet.top[1][w]);
-        l.enter(a, list, c0, c1);
-        l.sums(a, lt, 0.0f, list);
-        l.sum = wave_sum(l.sum);
-        if (lead) meet.sum[1][wid] = l.sum;
-        __syncthreads();
-        l.sum = 0.0;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) l.sum += meet.sum[1][w];
-        l.finish();
-        const float m = a.norm_in[2 * row];
-        const float ref = m == -INFINITY ? 0.0f : m;
-        const float per_sum = (float)exp(-(double)a.norm_in[2 * row + 1]);
-        const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
-        const float f = gt * per_sum;
-#pragma unroll
-        for (int v = 0; v < PART_VECS; ++v) {
-            const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
-            typename T::vec o;
-#pragma unroll
-            for (int i = 0; i < T::W; ++i) o[i] = T::round(l.some ? f * exp2_hw(expo(a, (float)h[v][i], ref)) : 0.0f);
-            if (c < whole - c0) store_vec<T>(g + c0 + c, o);
-        }
-        if (tail) g[ct] = T::round(l.some ? f * exp2_hw(expo(a, et, ref)) : 0.0f);
-        // what the workgroup has written so far is in memory, in front of what follows
-        __threadfence_block();
-        __syncthreads();
-        if (l.some) l.template patch<T>(a, list, g, c0, c1, ref, per_sum, gt);
-        __syncthreads();
+    for (int v = 0; v < PART_VECS; ++v) {
+        const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+        h[v] = fill_vec<T>(0.0f);
+        if (c < whole - c0) h[v] = load_vec<T>(z + c0 + c);
     }
+    if (tail) et = (float)z[ct];
+    l.clear(a, list);
+    float lt = wave_max(l.template take<T>(a, row, z, c0, c1, list));
+    if (lead) meet.top[1][wid] = lt;
+    __syncthreads();   // (everything has been read before anything is overwritten)
+#pragma unroll
+    for (int w = 0; w < NW; ++w) lt = fmaxf(lt, meet.top[1][w]);
+    l.enter(a, list, c0, c1);
+    l.sums(a, lt, 0.0f, list);
+    l.sum = wave_sum(l.sum);
+    if (lead) meet.sum[1][wid] = l.sum;
+    __syncthreads();
+    l.sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) l.sum += meet.sum[1][w];
+    l.finish();
+    const float m = a.norm_in[2 * row];
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float per_sum = (float)exp(-(double)a.norm_in[2 * row + 1]);
+    const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
+    const float f = gt * per_sum;
+#pragma unroll
+    for (int v = 0; v < PART_VECS; ++v) {
+        const uint32_t c = ((uint32_t)v * NT + threadIdx.x) * T::W;
+        typename T::vec o;
+#pragma unroll
+        for (int i = 0; i < T::W; ++i) o[i] = T::round(l.some ? f * exp2_hw(expo(a, (float)h[v][i], ref)) : 0.0f);
+        if (c < whole - c0) store_vec<T>(g + c0 + c, o);
+    }
+    if (tail) g[ct] = T::round(l.some ? f * exp2_hw(expo(a, et, ref)) : 0.0f);
+    // what the workgroup has written so far is in memory, in front of what follows
+    __threadfence_block();
+    __syncthreads();
+    if (l.some) l.template patch<T>(a, list, g, c0, c1, ref, per_sum, gt);
 }
 
-uint32_t grid_of(uint64_t n) { return (uint32_t)(n < (1u << 20) ? n : (1u << 20)); }
+// One workgroup a row, or a chunk of one, and a launch for every 2^20 of them (a kernel without a loop over rows keeps nothing
+// from one row to the next in registers, NV = 16 with the gradient 112 of them instead of 167).
+template <typename F>
+void for_rows(DistillArgs a, uint64_t groups_a_row, F&& launch) {
+    const uint32_t run = (uint32_t)(groups_a_row >= (1u << 20) ? 1u : (1u << 20) / groups_a_row);
+    for (uint64_t row = 0; row < a.n_rows; row += run) {
+        a.row0 = (uint32_t)row;
+        launch(a, dim3((uint32_t)(std::min<uint64_t>(run, a.n_rows - row) * groups_a_row)));
+    }
+}
 
 static_assert(F32by8::W == 8 && F16::W == 8 && BF16::W == 8 && PART_MAX % PART_STEP == 0, "a chunk fits the part kernels' registers");
 
@@ -506,22 +504,32 @@ void set_chunks(DistillArgs& a) {
 }
 
 template <typename T, int NT, int NV>
-void launch_row(const DistillArgs& a, hipStream_t st) {
-    if (a.grad) hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, true>), dim3(grid_of(a.n_rows)), dim3(NT), list_bytes(a, true), st, a);
-    else hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, false>), dim3(grid_of(a.n_rows)), dim3(NT), list_bytes(a, false), st, a);
+void launch_row(const DistillArgs& args, hipStream_t st) {
+    for_rows(args, 1, [&](const DistillArgs& a, dim3 grid) {
+        if (a.grad) hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, true>), grid, dim3(NT), list_bytes(a, true), st, a);
+        else hipLaunchKernelGGL((distill_row_kernel<T, NT, NV, false>), grid, dim3(NT), list_bytes(a, false), st, a);
+    });
 }
 
 template <typename T>
-void launch_grad(const DistillArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((distill_grad_kernel<T, 256>), dim3(grid_of((uint64_t)a.n_rows * a.n_chunks)), dim3(256), list_bytes(a, true), st, a);
+void launch_grad(const DistillArgs& args, hipStream_t st) {
+    for_rows(args, args.n_chunks, [&](const DistillArgs& a, dim3 grid) {
+        hipLaunchKernelGGL((distill_grad_kernel<T, 256>), grid, dim3(256), list_bytes(a, true), st, a);
+    });
 }
 
 template <typename T>
 void launch_loss(DistillArgs a, hipStream_t st) {
     if (a.n_cols <= ROW_MAX) {
-        // The fewest threads that hold the row, where there are rows enough to fill the chip (4096 x 4000 bf16 with the gradient:
-        // one wave a row 20.7 us, four 27.5; 64 x 4000: 8.1 and 6.7; 4096 x 32000: four waves 111 us, eight 164, sixteen 346).
+        // The fewest threads that hold the row, where there are rows enough to fill the chip (bf16 with the gradient, us: 4096 x
+        // 2000 one wave a row 14.2, four 17.7; 4096 x 8000 four waves 29.8, eight 36.4; 4096 x 20000 four waves 69, eight 79,
+        // sixteen 95 and more; 64 x 4000 one wave 8.1, four 6.8).
         const bool many = a.n_rows >= 1024u;
+        // (Very many rows of nearly what four waves hold: as 16-bit rows of eight waves three of them are on a CU at a time instead of
+        // four, and reads and writes get in each other's way less. 4096 x 32000 bf16 with the gradient 104 us, four waves 111;
+        // 8192 x 32000 191, 215; but 2000 x 29999 64, 60 and 4096 x 20000 79, 69.)
+        if constexpr (sizeof(typename T::elem) == 2)
+            if (a.n_cols > 24576u && a.n_cols <= 32768u && a.n_rows >= 2560u) return launch_row<T, 512, 8>(a, st);
         if (a.n_cols <= 512u) launch_row<T, 64, 1>(a, st);
         else if (a.n_cols <= 1024u) launch_row<T, 64, 2>(a, st);
         else if (a.n_cols <= 2048u && many) launch_row<T, 64, 4>(a, st);
@@ -534,8 +542,8 @@ void launch_loss(DistillArgs a, hipStream_t st) {
         else launch_row<T, 512, 16>(a, st);
         return;
     }
-    hipLaunchKernelGGL((distill_part_kernel<T, 256>), dim3(grid_of((uint64_t)a.n_rows * a.n_chunks)), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((distill_join_kernel<T, 256>), dim3(grid_of(a.n_rows)), dim3(256), list_bytes(a, false), st, a);
+    for_rows(a, a.n_chunks, [&](const DistillArgs& a, dim3 grid) { hipLaunchKernelGGL((distill_part_kernel<T, 256>), grid, dim3(256), 0, st, a); });
+    for_rows(a, 1, [&](const DistillArgs& a, dim3 grid) { hipLaunchKernelGGL((distill_join_kernel<T, 256>), grid, dim3(256), list_bytes(a, false), st, a); });
     if (a.grad) {
         a.norm_in = a.norm;
         launch_grad<T>(a, st);

@@ -30,6 +30,7 @@ struct Q8Args {
     uint64_t x_stride, residual_stride, sum_stride, q8_stride, values_stride;
     uint32_t n_rows, dim;
     float eps;
+    uint32_t row0;   // first row of a launch
 };
 
 // nearest(127 p / top), ties to even. inv = 127 / top has its own rounding, which could move a tie off the
@@ -142,9 +143,8 @@ __device__ __forceinline__ void row_scale(const Q8Args& a, double top, double ss
 
 // NT threads a row (16 lanes, a wave, or a workgroup), NV vectors of W elements a thread; the elements behind the last whole
 // vector: one each for the first few threads. NV == 0: the row does not fit the registers, it is read again for the
-// integers. (Tried: loads without a branch in front -- clamped to the row's last vector, results masked -- and the next
-// row's loads ahead of this row's work. Both need the raw vectors held beside the products, 152 registers instead of 84,
-// and what the occupancy loses is more: 16384 x 4096 bf16 130 us instead of 112, 1M x 384 f32 736 instead of 614.)
+// integers. What bounds it: 16384 x 4096 bf16 with residual, sum and values 111 us, 5.4 TB/s, what a large copy reaches. (Tried:
+// the loads of all vectors ahead of the arithmetic, 81 registers instead of 58: 120 us; 4000 x 12000 118 instead of 84.)
 template <typename T, bool NORM, int NT, int NV>
 __global__ void __launch_bounds__(NT < 256 ? 256 : NT) q8_rows_kernel(const Q8Args a) {
     typedef typename T::elem E;
@@ -152,89 +152,90 @@ __global__ void __launch_bounds__(NT < 256 ? 256 : NT) q8_rows_kernel(const Q8Ar
     constexpr int NW = NT / 64, W = T::W;
     constexpr int L = NT < 64 ? NT : 64;                   // lanes that reduce together
     constexpr uint32_t RPB = NT < 256 ? 256u / NT : 1u;    // rows a workgroup has at a time
-    __shared__ double sh[2][NW > 1 ? NW : 1][2];
+    __shared__ double sh[NW > 1 ? NW : 1][2];
     const uint32_t t = threadIdx.x % (NT < 256 ? NT : 1024);
     const E* const w = reinterpret_cast<const E*>(a.weight);
     const uint32_t whole = a.dim / W * W, et = whole + t;
     const bool tail = t < (uint32_t)W && et < a.dim;
-    uint32_t turn = 0;
-    for (uint64_t row = (uint64_t)blockIdx.x * RPB + (NT < 256 ? threadIdx.x / NT : 0u); row < a.n_rows;
-         row += (uint64_t)gridDim.x * RPB, turn ^= 1u) {
-        const E* const x = reinterpret_cast<const E*>(a.x) + row * a.x_stride;
-        const E* const res = a.residual ? reinterpret_cast<const E*>(a.residual) + row * a.residual_stride : nullptr;
-        E* const sum = a.sum ? reinterpret_cast<E*>(a.sum) + row * a.sum_stride : nullptr;
-        E* const values = a.values ? reinterpret_cast<E*>(a.values) + row * a.values_stride : nullptr;
-        int8_t* const q8 = a.q8 + row * a.q8_stride;
-        double top = 0.0, ss = 0.0;
-        double p[NV > 0 ? NV : 1][W], pt[1] = {0.0};
-        if constexpr (NV > 0) {
+    const uint64_t row = (uint64_t)a.row0 + (uint64_t)blockIdx.x * RPB + (NT < 256 ? threadIdx.x / NT : 0u);
+    if (row >= a.n_rows) return;   // (parts of a wave at most: a workgroup's row is always there)
+    const E* const x = reinterpret_cast<const E*>(a.x) + row * a.x_stride;
+    const E* const res = a.residual ? reinterpret_cast<const E*>(a.residual) + row * a.residual_stride : nullptr;
+    E* const sum = a.sum ? reinterpret_cast<E*>(a.sum) + row * a.sum_stride : nullptr;
+    E* const values = a.values ? reinterpret_cast<E*>(a.values) + row * a.values_stride : nullptr;
+    int8_t* const q8 = a.q8 + row * a.q8_stride;
+    double top = 0.0, ss = 0.0;
+    double p[NV > 0 ? NV : 1][W], pt[1] = {0.0};
+    if constexpr (NV > 0) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint32_t e = ((uint32_t)v * NT + t) * W;
-                if (e < whole) {
-                    products<T, NORM, W>(x, res, w, sum, e, p[v], ss);
+        for (int v = 0; v < NV; ++v) {
+            const uint32_t e = ((uint32_t)v * NT + t) * W;
+            if (e < whole) {
+                products<T, NORM, W>(x, res, w, sum, e, p[v], ss);
 #pragma unroll
-                    for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[v][i]));
-                }
+                for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[v][i]));
             }
-            if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, ss);
-        } else {
-            // (the sum is written in the second pass: it may go in place of an operand)
-            for (uint32_t e = t * W; e < whole; e += NT * W) {
-                products<T, NORM, W>(x, res, w, nullptr, e, p[0], ss);
-#pragma unroll
-                for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[0][i]));
-            }
-            if (tail) products<T, NORM, 1>(x, res, w, nullptr, et, pt, ss);
         }
-        top = __builtin_fmax(top, __builtin_fabs(pt[0]));
-        top = lanes_max<L>(top);
-        ss = lanes_sum<L>(ss);
-        if constexpr (NW > 1) {
-            // (two turns of the array: a wave that is ahead writes the next row's partials beside the ones still read)
-            if ((threadIdx.x & 63u) == 0) { sh[turn][threadIdx.x >> 6][0] = top; sh[turn][threadIdx.x >> 6][1] = ss; }
-            __syncthreads();
-            top = sh[turn][0][0];
-            ss = sh[turn][0][1];
+        if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, ss);
+    } else {
+        // (the sum is written in the second pass: it may go in place of an operand)
+        for (uint32_t e = t * W; e < whole; e += NT * W) {
+            products<T, NORM, W>(x, res, w, nullptr, e, p[0], ss);
 #pragma unroll
-            for (int i = 1; i < NW; ++i) { top = __builtin_fmax(top, sh[turn][i][0]); ss += sh[turn][i][1]; }
+            for (int i = 0; i < W; ++i) top = __builtin_fmax(top, __builtin_fabs(p[0][i]));
         }
-        double inv;
-        float scale;
-        row_scale<NORM>(a, top, ss, inv, scale);
-        if (t == 0) a.scale[row] = scale;
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint32_t e = ((uint32_t)v * NT + t) * W;
-                if (e < whole) store_q8<T, W>(q8, values, e, p[v], inv, top, scale);
-            }
-        } else {
-            double again = 0.0;
-            for (uint32_t e = t * W; e < whole; e += NT * W) {
-                products<T, NORM, W>(x, res, w, sum, e, p[0], again);
-                store_q8<T, W>(q8, values, e, p[0], inv, top, scale);
-            }
-            if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, again);
-        }
-        if (tail) store_q8<T, 1>(q8, values, et, pt, inv, top, scale);
+        if (tail) products<T, NORM, 1>(x, res, w, nullptr, et, pt, ss);
     }
+    top = __builtin_fmax(top, __builtin_fabs(pt[0]));
+    top = lanes_max<L>(top);
+    ss = lanes_sum<L>(ss);
+    if constexpr (NW > 1) {
+        if ((threadIdx.x & 63u) == 0) { sh[threadIdx.x >> 6][0] = top; sh[threadIdx.x >> 6][1] = ss; }
+        __syncthreads();
+        top = sh[0][0];
+        ss = sh[0][1];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) { top = __builtin_fmax(top, sh[i][0]); ss += sh[i][1]; }
+    }
+    double inv;
+    float scale;
+    row_scale<NORM>(a, top, ss, inv, scale);
+    if (t == 0) a.scale[row] = scale;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const uint32_t e = ((uint32_t)v * NT + t) * W;
+            if (e < whole) store_q8<T, W>(q8, values, e, p[v], inv, top, scale);
+        }
+    } else {
+        double again = 0.0;
+        for (uint32_t e = t * W; e < whole; e += NT * W) {
+            products<T, NORM, W>(x, res, w, sum, e, p[0], again);
+            store_q8<T, W>(q8, values, e, p[0], inv, top, scale);
+        }
+        if (tail) products<T, NORM, 1>(x, res, w, sum, et, pt, again);
+    }
+    if (tail) store_q8<T, 1>(q8, values, et, pt, inv, top, scale);
 }
 
-// NV: vectors of eight elements, whatever the type
+// NV: vectors of eight elements, whatever the type. A launch for every 2^20 workgroups: a kernel without a loop over rows keeps
+// nothing from one row to the next in registers.
 template <typename T, bool NORM, int NT, int NV>
 void launch_one(const Q8Args& a, hipStream_t st) {
-    constexpr uint32_t rpb = NT < 256 ? 256u / NT : 1u, most = 1u << 20;
-    const uint64_t blocks = ((uint64_t)a.n_rows + rpb - 1) / rpb;
-    const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
-    hipLaunchKernelGGL((q8_rows_kernel<T, NORM, NT, NV * 8 / T::W>), dim3(grid), dim3(NT < 256 ? 256 : NT), 0, st, a);
+    constexpr uint32_t rpb = NT < 256 ? 256u / NT : 1u, run = rpb << 20;
+    Q8Args r = a;
+    for (uint64_t row = 0; row < a.n_rows; row += run) {
+        const uint64_t rows = a.n_rows - row < run ? a.n_rows - row : run;
+        r.row0 = (uint32_t)row;
+        hipLaunchKernelGGL((q8_rows_kernel<T, NORM, NT, NV * 8 / T::W>), dim3((uint32_t)((rows + rpb - 1) / rpb)), dim3(NT < 256 ? 256 : NT), 0, st, r);
+    }
 }
 
 template <typename T, bool NORM>
 void launch_type(const Q8Args& a, hipStream_t st) {
-    // As few lanes a row as hold it: more bytes of a lane in flight, fewer steps of the reductions. us, by lanes a row:
-    // 300k x 384 bf16 norm 16 lanes 185, 32 235, 64 350; 200k x 768 bf16 norm 32 lanes 241, 64 299; 30k x 1500 bf16 norm
-    // 64 lanes 86, 256 112-128; 16384 x 4096 bf16 norm 256 threads 112, 512 182.
+    // As few lanes a row as hold it: more bytes of a lane in flight, fewer steps of the reductions. us, by lanes a row, bf16 with
+    // the norm: 300k x 384 16 lanes 196, 32 214, 64 284; 200k x 768 32 lanes 252, 64 274; 30k x 1500 64 lanes 87, 256 107;
+    // 16384 x 4096 256 threads 111, 512 137; 4000 x 12000 1024 threads 84, 512 86, 256 91; 8000 x 8192 256 or 512 threads 108.
     if (a.dim <= 128u) launch_one<T, NORM, 16, 1>(a, st);
     else if (a.dim <= 256u) launch_one<T, NORM, 16, 2>(a, st);
     else if (a.dim <= 384u) launch_one<T, NORM, 16, 3>(a, st);
@@ -304,7 +305,7 @@ trag_status trag_rmsnorm_q8_device(const void* d_x, uint64_t x_stride, const voi
         const char* who = "trag_rmsnorm_q8_device";
         if (n_rows == 0) return TRAG_OK;
         const Q8Args a{d_x, d_residual, d_weight, d_sum, d_q8, d_scale, d_values, x_stride, residual_stride, sum_stride,
-                       q8_stride, values_stride, n_rows, dim, eps};
+                       q8_stride, values_stride, n_rows, dim, eps, 0};
         trag_status ts = check_rows(who, a, dtype);
         if (ts != TRAG_OK) return ts;
         if (!(eps >= 0.0f) || !(eps - eps == 0.0f)) return set_error(TRAG_INVALID_ARG, std::string(who) + ": eps must be finite and not negative");
@@ -323,7 +324,7 @@ trag_status trag_quantize_q8_device(const void* d_x, uint64_t x_stride, uint32_t
         const char* who = "trag_quantize_q8_device";
         if (n_rows == 0) return TRAG_OK;
         const Q8Args a{d_x, nullptr, nullptr, nullptr, d_q8, d_scale, d_values, x_stride, 0, 0, q8_stride, values_stride,
-                       n_rows, dim, 0.0f};
+                       n_rows, dim, 0.0f, 0};
         trag_status ts = check_rows(who, a, dtype);
         if (ts != TRAG_OK) return ts;
         OpDevice on(who, hip_stream, {d_x, d_q8, d_scale, d_values});
