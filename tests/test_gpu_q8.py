@@ -228,6 +228,27 @@ def _expect(a, b, sa, sb, dt):
     return c.to(dt)
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,dim", [(r, d) for r in (1030, 2051, 4103) for d in (100, 201, 300, 505, 700, 1000, 1300, 2001)] + [(520, 5001), (1030, 9000)])
+def test_forms_for_many_rows(trag, t, rows, dim):
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(rows + dim)
+    dt = _types()[t]
+    xb, x = _strided(rows, dim, 3, dt, 1)
+    x.copy_(torch.randn((rows, dim), generator=g, device="cuda"))
+    r = torch.randn((rows, dim), generator=g, device="cuda").to(dt)
+    w = (1 + 0.2 * torch.randn(dim, generator=g, device="cuda")).to(dt)
+    want = (x.float() + r.float()).to(dt)
+    x0 = x.clone()
+    qb, q8 = _strided(rows, dim, 5, torch.int8, 1)
+    scale = torch.full((rows + 3,), float(FILL), device="cuda")
+    values = torch.empty((rows, dim), dtype=dt, device="cuda")
+    _run_norm(trag, t, x, r, w, 1e-5, x, q8, scale, values)      # (the sum in place)
+    _check_rows(x0, r, w, 1e-5, q8, scale[:rows])
+    assert torch.equal(x, want) and torch.equal(values, (q8.float() * scale[:rows, None]).to(dt))
+    assert _untouched(xb, x, 1) and _untouched(qb, q8, 1) and (scale[rows:] == FILL).all()
+
+
 def test_more_rows_than_one_launch_takes(trag):
     torch = _torch()
     rows = 2 ** 24 + 35

@@ -12,7 +12,7 @@
 // roundings; with them it is a function of the inputs alone.
 //
 // Bound by HBM: per element a read of x (and the residual), a write of the sum, of q and, if asked for, of
-// the values they stand for. 16 lanes to a wave a row up to 2048 elements, one workgroup a row beyond; a row too
+// the values they stand for. 16 lanes to a workgroup a row, by its length and how many rows there are; a row too
 // long for registers (over 32768 elements) is read twice, the second time from the caches.
 #include "trag_ops.h"
 
@@ -233,22 +233,44 @@ void launch_one(const Q8Args& a, hipStream_t st) {
 
 template <typename T, bool NORM>
 void launch_type(const Q8Args& a, hipStream_t st) {
-    // As few lanes a row as hold it: more bytes of a lane in flight, fewer steps of the reductions. us, by lanes a row, bf16 with
-    // the norm: 300k x 384 16 lanes 196, 32 214, 64 284; 200k x 768 32 lanes 252, 64 274; 30k x 1500 64 lanes 87, 256 107;
-    // 16384 x 4096 256 threads 111, 512 137; 4000 x 12000 1024 threads 84, 512 86, 256 91; 8000 x 8192 256 or 512 threads 108.
-    if (a.dim <= 128u) launch_one<T, NORM, 16, 1>(a, st);
-    else if (a.dim <= 256u) launch_one<T, NORM, 16, 2>(a, st);
-    else if (a.dim <= 384u) launch_one<T, NORM, 16, 3>(a, st);
-    else if (a.dim <= 512u) launch_one<T, NORM, 32, 2>(a, st);
-    else if (a.dim <= 768u) launch_one<T, NORM, 32, 3>(a, st);
-    else if (a.dim <= 1024u) launch_one<T, NORM, 64, 2>(a, st);
-    else if (a.dim <= 1536u) launch_one<T, NORM, 64, 3>(a, st);
-    else if (a.dim <= 2048u) launch_one<T, NORM, 64, 4>(a, st);
-    else if (a.dim <= 4096u) launch_one<T, NORM, 256, 2>(a, st);
-    else if (a.dim <= 8192u) launch_one<T, NORM, 256, 4>(a, st);
-    else if (a.dim <= 16384u) launch_one<T, NORM, 1024, 2>(a, st);
-    else if (a.dim <= 32768u) launch_one<T, NORM, 1024, 4>(a, st);
-    else launch_one<T, NORM, 1024, 0>(a, st);
+    // Many rows: as few lanes a row as hold it -- more bytes of a lane in flight, fewer steps of the reductions -- and twice as many
+    // in f32, whose vectors hold four elements. us, by lanes a row, 16-bit with the norm: 300k x 384 16 lanes 196, 32 214, 64 284;
+    // 200k x 768 32 lanes 252, 64 274; 30k x 1500 64 lanes 87, 256 107; 16384 x 4096 256 threads 111, 512 137; 4000 x 12000 1024
+    // threads 84, 512 86, 256 91. f32 as it is: 1M x 384 16 lanes 615, 64 600; 150k x 2048 64 lanes 507, 256 458; 60k x 4096 256
+    // threads 386, 512 369.
+    // Few rows: as many lanes as there is work for, since a row's time is its longest lane's (us of the kernel among others of its
+    // kind, 16-bit with the norm: 1 x 384 64 lanes 2.8, 16 lanes 5.2, 1000 rows 3.5, 6.0, 6000 rows 11, 9.4; 400 x 768 256 threads
+    // 4.2, 64 lanes 4.9, 32 lanes 5.9; 1000 x 2048 256 threads 8.1, 64 lanes 9.9, 2000 rows 12.5, 12.4; 1 x 6000 512 threads
+    // 4.4, 256 5.1, 1000 rows 13.2, 12.9).
+    const bool few = a.n_rows <= 1024u, some = a.n_rows <= 4096u;
+    if constexpr (T::W == 4) {
+        if (a.dim <= 128u) some ? launch_one<T, NORM, 32, 1>(a, st) : launch_one<T, NORM, 16, 1>(a, st);
+        else if (a.dim <= 256u) some ? launch_one<T, NORM, 64, 1>(a, st) : launch_one<T, NORM, 32, 1>(a, st);
+        else if (a.dim <= 512u) launch_one<T, NORM, 64, 1>(a, st);
+        else if (a.dim <= 1024u && !few) launch_one<T, NORM, 64, 2>(a, st);
+        else if (a.dim <= 2048u) launch_one<T, NORM, 256, 1>(a, st);
+        else if (a.dim <= 4096u) launch_one<T, NORM, 512, 1>(a, st);
+        else if (a.dim <= 8192u) launch_one<T, NORM, 512, 2>(a, st);
+        else if (a.dim <= 16384u) launch_one<T, NORM, 1024, 2>(a, st);
+        else if (a.dim <= 32768u) launch_one<T, NORM, 1024, 4>(a, st);
+        else launch_one<T, NORM, 1024, 0>(a, st);
+    } else {
+        if (a.dim <= 128u) launch_one<T, NORM, 16, 1>(a, st);
+        else if (a.dim <= 256u) some ? launch_one<T, NORM, 32, 1>(a, st) : launch_one<T, NORM, 16, 2>(a, st);
+        else if (a.dim <= 512u && some) launch_one<T, NORM, 64, 1>(a, st);
+        else if (a.dim <= 384u) launch_one<T, NORM, 16, 3>(a, st);
+        else if (a.dim <= 512u) launch_one<T, NORM, 32, 2>(a, st);
+        else if (a.dim <= 2048u && few) launch_one<T, NORM, 256, 1>(a, st);
+        else if (a.dim <= 768u && a.n_rows > 2048u) launch_one<T, NORM, 32, 3>(a, st);
+        else if (a.dim <= 1024u) launch_one<T, NORM, 64, 2>(a, st);
+        else if (a.dim <= 1536u) launch_one<T, NORM, 64, 3>(a, st);
+        else if (a.dim <= 2048u) launch_one<T, NORM, 64, 4>(a, st);
+        else if (a.dim <= 4096u) launch_one<T, NORM, 256, 2>(a, st);
+        else if (a.dim <= 8192u) a.n_rows <= 512u ? launch_one<T, NORM, 512, 2>(a, st) : launch_one<T, NORM, 256, 4>(a, st);
+        else if (a.dim <= 16384u) launch_one<T, NORM, 1024, 2>(a, st);
+        else if (a.dim <= 32768u) launch_one<T, NORM, 1024, 4>(a, st);
+        else launch_one<T, NORM, 1024, 0>(a, st);
+    }
 }
 
 template <bool NORM>
