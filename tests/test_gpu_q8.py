@@ -284,6 +284,24 @@ def test_product_is_exact(trag, m, n, dim, t):
         assert _untouched(ob, out)
 
 
+@pytest.mark.parametrize("m,n,dim", [(3421, 2373, 432), (791, 10075, 438), (489, 1399, 409), (2377, 201, 405), (65, 33717, 624), (2325, 2467, 429),
+                                     (915, 261, 704), (2927, 1221, 426), (273, 997, 400), (113, 1067, 432), (1129, 101, 576), (701, 397, 551),
+                                     (2563, 405, 400), (111, 297, 448), (69, 28779, 480), (19, 23123, 496), (855, 303, 411), (331, 8661, 1184),
+                                     (3491, 1705, 34), (2997, 495, 33), (611, 4355, 33), (4, 65, 192), (177, 161, 320), (13, 35, 1111)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_product_in_every_tile(trag, m, n, dim, t):
+    """Sizes between them reach every tile, with rows at multiples of 16 bytes and at any byte."""
+    torch = _torch()
+    g = torch.Generator(device="cuda").manual_seed(m * 7 + n)
+    for pad, offset in ((0, 0), (5, 1)):
+        a, b = _int8(m, dim, pad, offset, g, True), _int8(n, dim, pad, offset, g, True)
+        sa, sb = torch.rand(m, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda")
+        ob, out = _strided(m, n, 3, _types()[t])
+        _product(trag, a, b, sa, sb, out, t)
+        assert torch.equal(out, _expect(a, b, sa, sb, _types()[t])), (pad, offset)
+        assert _untouched(ob, out)
+
+
 def test_product_without_scales_and_with_nan_scales(trag):
     torch = _torch()
     g = torch.Generator(device="cuda").manual_seed(5)

@@ -70,11 +70,11 @@ __device__ __forceinline__ TilePos tile_of(uint32_t b, uint32_t m_tiles, uint32_
     return {g0 + in % rows, in / rows, true};
 }
 
-// ---- small tiles, straight into matrix fragments: a wave takes 16 MT rows of a and 16 NT rows of b; lane l holds 16
-// bytes of row l % 16 from k = 16 (l / 16) on, so a wave-instruction reads 64 consecutive bytes of each of 16
-// rows. Nothing goes through LDS but the joining of partial sums where WK waves share one tile's terms, which
-// is what fills the chip when there are few tiles. U: 64-byte steps whose loads are in flight together; the
-// next U are asked for before the current ones are used. WN: tiles side by side in one workgroup.
+// ---- rows shorter than a chunk, or 2^24 bytes and more apart, straight into matrix fragments: a wave takes 16 MT rows of a
+// and 16 NT rows of b; lane l holds 16 bytes of row l % 16 from k = 16 (l / 16) on, so a wave-instruction reads 64 consecutive
+// bytes of each of 16 rows. Nothing goes through LDS but the joining of partial sums where WK waves share one tile's terms. U:
+// 64-byte steps whose loads are in flight together; the next U are asked for before the current ones are used. WN: tiles side
+// by side in one workgroup.
 template <typename T, int MT, int NT, int WK, int WN, int U, bool SHORT>
 __global__ void __launch_bounds__(64 * WK * WN) mm_direct_kernel(const MmArgs p) {
     typedef typename T::elem E;
@@ -512,37 +512,40 @@ bool dma_fits(const MmArgs& p) {
     return p.dim % 16u == 0 && p.lda % 16u == 0 && p.ldb % 16u == 0 && aligned_to(p.a, 16) && aligned_to(p.b, 16);
 }
 
-bool quads(const MmArgs& p) { return p.lda % 4u == 0 && p.ldb % 4u == 0 && aligned_to(p.a, 4) && aligned_to(p.b, 4); }
-
 // Which tile. Every form gives the same bits, so the choice is one of time alone: the one with the least
 //   max(rounds (fix + per * steps a group of waves does), operands and output / 6 TB/s + what tiles read again / 16 TB/s),
-// rounds = tiles over what 256 CUs hold at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
-// up (12 TB/s for rows at any byte). The constants are fitted to these times (us; bf16 output; aligned rows, m x n x dim):
-//   16 x 4096 x 4096   16 x 64 tiles in 4 groups of waves  7.2    in 1  16.3    32 x 64 in 4   7.7
-//   64 x 4096 x 4096   32 x 64 in 4   8.0    64 x 64 in 2   9.7    in 1  17.5
-//   256 x 4096 x 4096  64 x 64 in 2  10.3    in 1  18.0    128 x 128 in 2  20.1    in 1  24.0
+// rounds = tiles over what 256 CUs work on at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
+// up (12 TB/s for rows at any byte). The constants are fitted, form by form, to the times of 1900 products of random sizes
+// (1 to 4096 by 64 to 1M by 32 to 8192); over 1000 others the choice takes 1.8 % longer than the best form on average, 11 % in
+// the worst twentieth. Some of the times (us of the kernel among others of its kind; bf16 output; aligned rows, m x n x dim):
+//   16 x 4096 x 4096   16 x 16 tiles in 8 groups of waves  6.3    16 x 32 in 4  6.4    16 x 64 in 4  7.5    in 1  16.6
+//   8 x 2048 x 8192    16 x 16 in 8   6.4    16 x 32 in 4   8.2    16 x 64 in 4  10.5    in 1  30.3
+//   100 x 1000 x 4096  16 x 32 in 4   6.2    16 x 64 in 4   7.4    32 x 64 in 4   8.3    16 x 16 in 8   8.4
+//   256 x 4096 x 4096  64 x 64 in 2  10.6    32 x 64 in 4  11.3    in 1  18.0    128 x 128 in 2  20.1    in 1  24.0
 //   1024 x 4096 x 4096 128 x 128 in 2  22.7    64 x 128  25.0    128 x 128 in 1  25.9    64 x 64 in 1  28.7    256 x 256  44.5
 //   4096 x 16384 x 4096  256 x 256  235    128 x 128 in 1  290
 //   1 x 1M x 384  16 x 64 in 1  66    64 x 1M x 384  64 x 128  102, 64 x 64  108    128 x 1M x 384  128 x 128  136, 64 x 64  180
 // and for rows at any byte (through registers):
-//   37 x 50021 x 777  64 x 128  12.2, 64 x 64  13.5    512 x 4096 x 4001  64 x 64  22.6, 64 x 128  23.0, 128 x 128  28.8
-//   1024 x 4096 x 4001  128 x 128  29.9, 64 x 128  33.1, 64 x 64  42.1    4096 x 8192 x 4001  256 x 256  150, 128 x 128  189
-enum TileForm { T16, T16G4, T32, T32G4, T64, T64G2, T64G4, T64x128, T128, T128G2, T256, N_FORMS };
+//   3 x 887 x 4404  16 x 16 in 8  5.2, 32 x 64 in 4  8.7    37 x 50021 x 777  64 x 128  12.2, 64 x 64  13.5
+//   512 x 4096 x 4001  64 x 64  22.6, 64 x 128  23.0, 128 x 128  28.8    4096 x 8192 x 4001  256 x 256  150, 128 x 128  189
+enum TileForm { T16x16G8, T16x32G4, T16, T16G4, T32, T32G4, T64, T64G2, T64x128, T128, T128G2, T256, N_FORMS };
 struct FormCost {
     uint16_t bm, bn, groups, threads;
-    uint16_t held;             // workgroups a CU holds (0: this form is not built)
+    uint16_t held;             // workgroups a CU works on at once (0: this form is not built)
     float fix, lo, hi;
 };
 constexpr FormCost DMA_COST[N_FORMS] = {
-    {16, 64, 1, 128, 5, 3.7f, 0.30f, 0.38f},   {16, 64, 4, 512, 1, 2.4f, 0.28f, 0.30f}, {32, 64, 1, 128, 6, 5.0f, 0.45f, 0.50f},
-    {32, 64, 4, 512, 1, 1.9f, 0.48f, 0.52f},   {64, 64, 1, 256, 5, 3.0f, 0.36f, 0.70f}, {64, 64, 2, 512, 1, 1.8f, 0.38f, 0.40f},
-    {64, 64, 4, 1024, 0, 0.0f, 0.0f, 0.0f},    {64, 128, 1, 256, 3, 3.0f, 0.45f, 0.76f}, {128, 128, 1, 256, 2, 3.8f, 0.50f, 0.90f},
-    {128, 128, 2, 512, 1, 4.6f, 0.85f, 0.98f}, {256, 256, 1, 512, 1, 7.5f, 1.30f, 1.60f}};
+    {16, 16, 8, 512, 1, 0.83f, 0.26f, 0.66f},   {16, 32, 4, 512, 1, 0.98f, 0.24f, 0.51f},
+    {16, 64, 1, 128, 5, 0.64f, 0.28f, 0.66f},   {16, 64, 4, 512, 1, 1.13f, 0.38f, 0.73f},   {32, 64, 1, 128, 6, 0.94f, 0.30f, 1.04f},
+    {32, 64, 4, 512, 1, 1.36f, 0.48f, 0.89f},   {64, 64, 1, 256, 5, 1.04f, 0.31f, 1.20f},   {64, 64, 2, 512, 1, 1.53f, 0.34f, 0.60f},
+    {64, 128, 1, 256, 3, 1.73f, 0.43f, 1.15f},  {128, 128, 1, 256, 2, 2.60f, 0.55f, 1.14f},
+    {128, 128, 2, 512, 1, 3.12f, 0.92f, 1.42f}, {256, 256, 1, 512, 1, 4.93f, 1.21f, 1.78f}};
 constexpr FormCost ANY_COST[N_FORMS] = {
-    {16, 64, 1, 128, 8, 2.7f, 0.43f, 0.60f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},   {32, 64, 1, 128, 6, 2.6f, 0.46f, 0.78f},
-    {32, 64, 4, 512, 1, 2.2f, 1.03f, 1.12f},   {64, 64, 1, 256, 5, 1.7f, 0.30f, 1.38f}, {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
-    {64, 64, 4, 1024, 1, 1.6f, 1.28f, 1.43f},  {64, 128, 1, 256, 3, 2.6f, 0.30f, 1.26f}, {128, 128, 1, 256, 2, 3.2f, 0.50f, 1.36f},
-    {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},   {256, 256, 1, 512, 1, 6.0f, 1.80f, 2.20f}};
+    {16, 16, 8, 512, 1, 0.38f, 0.70f, 0.72f},   {16, 32, 4, 512, 1, 0.35f, 0.62f, 0.51f},
+    {16, 64, 1, 128, 8, 0.91f, 0.34f, 1.70f},   {16, 64, 4, 512, 0, 0.0f, 0.0f, 0.0f},      {32, 64, 1, 128, 6, 1.22f, 0.36f, 1.62f},
+    {32, 64, 4, 512, 1, 1.23f, 0.86f, 1.43f},   {64, 64, 1, 256, 5, 1.54f, 0.36f, 1.85f},   {64, 64, 2, 512, 0, 0.0f, 0.0f, 0.0f},
+    {64, 128, 1, 256, 3, 2.18f, 0.53f, 1.73f},  {128, 128, 1, 256, 2, 3.07f, 0.81f, 1.65f},
+    {128, 128, 2, 512, 0, 0.0f, 0.0f, 0.0f},    {256, 256, 1, 512, 1, 5.20f, 1.86f, 2.40f}};
 
 int choose_form(const MmArgs& p, bool dma, uint32_t out_bytes) {
     constexpr double CUS = 256.0;
@@ -575,15 +578,11 @@ void launch_mm(const MmArgs& p, hipStream_t st) {
     // (the tiles' offsets from their first row are 32 bits, over 255 rows at most)
     if (p.lda >= (1u << 24) || p.ldb >= (1u << 24)) return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
     const bool dma = dma_fits(p);
-    // Rows at any byte, few enough for a workgroup of its own on a CU for every 16 x 16 sums, and long: fragments straight from
-    // memory, eight waves a tile's terms. us, and the best of the tiles: rows at multiples of 4, 16 x 2000 x 1001 5.2, 5.6;
-    // x 3001 5.7, 7.4; x 7550 10.7, 13.2; at odd bytes 5.9, 6.3; 10.1, 11.3; 26.3, 20.9, so not those; more rows, 16 x 8000 x 3001
-    // 9.1, 9.6 and at odd bytes 16.5, 11.9. Shorter rows take the time of the launch either way.
-    if (!dma && p.dim >= 512u && (uint64_t)((p.m + 15u) / 16u) * (((uint64_t)p.n + 15u) / 16u) <= 256u && (p.dim <= 4096u || quads(p)))
-        return launch_direct<T, 1, 1, 8, 1, 4>(p, st);
     const int form = choose_form(p, dma, sizeof(typename T::elem));
     if (dma) {
         switch (form) {
+            case T16x16G8: return launch_tile<T, 1, 1, 1, 1, 8, 4, true>(p, st);
+            case T16x32G4: return launch_tile<T, 1, 2, 1, 1, 4, 4, true>(p, st);
             case T16: return launch_tile<T, 1, 2, 1, 2, 1, 2, true>(p, st);
             case T16G4: return launch_tile<T, 1, 2, 1, 2, 4, 3, true>(p, st);
             case T32: return launch_tile<T, 1, 2, 2, 2, 1, 2, true>(p, st);
@@ -597,11 +596,12 @@ void launch_mm(const MmArgs& p, hipStream_t st) {
         }
     }
     switch (form) {
+        case T16x16G8: return launch_tile<T, 1, 1, 1, 1, 8, 2, false>(p, st);
+        case T16x32G4: return launch_tile<T, 1, 2, 1, 1, 4, 2, false>(p, st);
         case T16: return launch_tile<T, 1, 2, 1, 2, 1, 2, false>(p, st);
         case T32: return launch_tile<T, 1, 2, 2, 2, 1, 2, false>(p, st);
         case T32G4: return launch_tile<T, 1, 2, 2, 2, 4, 2, false>(p, st);
         case T64: return launch_tile<T, 2, 2, 2, 2, 1, 2, false>(p, st);
-        case T64G4: return launch_tile<T, 2, 2, 2, 2, 4, 2, false>(p, st);
         case T64x128: return launch_tile<T, 2, 2, 2, 4, 1, 2, false>(p, st);
         case T128: return launch_tile<T, 2, 2, 4, 4, 1, 2, false>(p, st);
         default: return launch_tile<T, 4, 2, 4, 8, 1, 2, false>(p, st);
