@@ -521,9 +521,10 @@ void launch_grad(const DistillArgs& args, hipStream_t st) {
 template <typename T>
 void launch_loss(DistillArgs a, hipStream_t st) {
     if (a.n_cols <= ROW_MAX) {
-        // The fewest threads that hold the row, where there are rows enough to fill the chip (bf16 with the gradient, us: 4096 x
-        // 2000 one wave a row 14.2, four 17.7; 4096 x 8000 four waves 29.8, eight 36.4; 4096 x 20000 four waves 69, eight 79,
-        // sixteen 95 and more; 64 x 4000 one wave 8.1, four 6.8).
+        // The fewest threads that hold the row, where there are rows enough to fill the chip (with the gradient, us: 5000 x 2000 bf16
+        // one wave a row 15.8, two 16.9, four 20.4; 5000 x 4000 two waves 23.3, one 23.4, four 26.1, f32 43.8, 46.0, 41.0; 5000 x
+        // 8000 bf16 four waves 37.6, two 43.6, eight 45.8; 4096 x 20000 four waves 69, eight 79); few rows of two vectors a thread
+        // (64 x 4000 four waves 6.6, two 6.9, one 7.9).
         const bool many = a.n_rows >= 1024u;
         // (Very many rows of nearly what four waves hold: as 16-bit rows of eight waves three of them are on a CU at a time instead of
         // four, and reads and writes get in each other's way less. 4096 x 32000 bf16 with the gradient 104 us, four waves 111;
@@ -534,7 +535,7 @@ void launch_loss(DistillArgs a, hipStream_t st) {
         else if (a.n_cols <= 1024u) launch_row<T, 64, 2>(a, st);
         else if (a.n_cols <= 2048u && many) launch_row<T, 64, 4>(a, st);
         else if (a.n_cols <= 2048u) launch_row<T, 128, 2>(a, st);
-        else if (a.n_cols <= 4096u && many) launch_row<T, 64, 8>(a, st);
+        else if (a.n_cols <= 4096u && many) launch_row<T, 128, 4>(a, st);
         else if (a.n_cols <= 4096u) launch_row<T, 256, 2>(a, st);
         else if (a.n_cols <= 8192u) launch_row<T, 256, 4>(a, st);
         else if (a.n_cols <= 16384u) launch_row<T, 256, 8>(a, st);
