@@ -9,7 +9,7 @@
 // gradient needs the row again. Bound by HBM: one read of the logits for the loss, one read and one write
 // for a gradient. Rows of up to 65536 columns stay in registers between the sum and the gradient; longer rows
 // are cut into chunks, each in the registers of one workgroup, whose partial (m, sum) pairs are joined by a second
-// launch, and which read the logits again for a gradient.
+// launch, the gradient's where there is one, which reads the logits again.
 //
 // Exponentials go through exp2 of (z - m) log2(e) / T: the difference first, so that rows at the type's lowest
 // value, whose product with 1 / T would overflow, still come out as the distribution they are. Sums over a
@@ -35,6 +35,7 @@ constexpr uint32_t PART_STEP = 2048;       // a chunk of a long row is a multipl
 // ... and at most what 256 threads hold as four vectors each (gradient of 4096 x 32000 bf16: 102 us, 5.1 TB/s; two vectors
 // 125, eight 102; reading the logits where each is needed 116)
 constexpr int PART_VECS = 4;
+constexpr uint32_t JOIN_MAX = 1024u;       // chunks of a row whose parts the gradient's workgroups join themselves
 constexpr uint32_t PART_MAX = 256u * 8u * PART_VECS;
 
 struct DistillArgs {
@@ -47,7 +48,7 @@ struct DistillArgs {
     const float* norm_in;     // the same, for the gradient alone
     const float* weight;      // per row, null: 1
     void* grad;
-    float* parts;             // 2 per row and chunk
+    float* parts;             // 2 per row and chunk, behind them 3 per row (list_part)
     uint64_t z_stride, grad_stride;
     uint32_t n_rows, n_cols, k, chunk, n_chunks;
     uint32_t row0;            // first row of a launch
@@ -321,8 +322,13 @@ __global__ void __launch_bounds__(NT, NT == 512 && sizeof(typename T::elem) == 2
     if (threadIdx.x == 0) write_row(a, row, m, sum, l);
 }
 
-// (max, sum) of one chunk of one row; a chunk is at most PART_VECS vectors a thread
-template <typename T, int NT>
+// What a row's list comes to before the row's maximum is known, behind the parts: a double, the sum of
+// e ((t - max t) - (z_id - zl)), and zl, the list's largest logit -- differences of logits, which lose nothing where the logits are huge.
+__device__ __forceinline__ float* list_part(const DistillArgs& a, uint64_t row) { return a.parts + 2 * (uint64_t)a.n_rows * a.n_chunks + 3 * row; }
+
+// (max, sum) of one chunk of one row; a chunk is at most PART_VECS vectors a thread. LIST: a row's first chunk does the list's
+// part of the loss too, while the logits are what they were (a gradient may go in their place).
+template <typename T, int NT, bool LIST>
 __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     typedef typename T::elem E;
     constexpr int NW = NT / 64;
@@ -331,6 +337,11 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     const bool lead = (threadIdx.x & 63u) == 0u;
     const uint64_t part = (uint64_t)a.row0 * a.n_chunks + blockIdx.x, row = part / a.n_chunks;
     const uint64_t c0 = (part % a.n_chunks) * a.chunk;
+    extern __shared__ uint32_t lds[];
+    const List list(a, lds);
+    Teacher<NT> l;
+    const bool first = LIST && c0 == 0;   // (of the whole workgroup)
+    if (first) l.ask(a, row);
     const uint32_t n = (uint32_t)min((uint64_t)a.chunk, a.n_cols - c0);
     const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride + c0;
     const uint32_t whole = n / T::W * T::W, ct = whole + threadIdx.x;   // (the columns behind the last whole vector, one each)
@@ -343,6 +354,33 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
         if (c < whole) h[v] = load_vec<T>(z + c);
     }
     if (threadIdx.x < (uint32_t)T::W && ct < n) et = (float)z[ct];
+    if constexpr (LIST) {
+        if (first) {
+            float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list)), zl = -INFINITY;
+            for (uint32_t j = threadIdx.x; j < a.k; j += NT)
+                if (list.id[j] != NO_ID) zl = fmaxf(zl, list.z[j]);
+            zl = wave_max(zl);
+            if (lead) { meet.top[0][wid] = zl; meet.top[1][wid] = lt; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; ++w) { zl = fmaxf(zl, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
+            if (zl == -INFINITY) zl = 0.0f;
+            l.sums(a, lt, zl, list);
+            l.cross = wave_sum(l.cross);
+            if (lead) meet.sum[1][wid] = l.cross;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                l.cross = 0.0;
+#pragma unroll
+                for (int w = 0; w < NW; ++w) l.cross += meet.sum[1][w];
+                float* const to = list_part(a, row);   // (4-byte aligned: the two words of a double)
+                const uint64_t bits = __builtin_bit_cast(uint64_t, l.cross);
+                to[0] = __builtin_bit_cast(float, (uint32_t)bits);
+                to[1] = __builtin_bit_cast(float, (uint32_t)(bits >> 32));
+                to[2] = zl;
+            }
+        }
+    }
     float m = et;
 #pragma unroll
     for (int v = 0; v < PART_VECS; ++v)
@@ -372,6 +410,26 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
     }
 }
 
+// this thread's part of a row's chunks: their maximum, and their sums brought to the row's maximum
+template <int NT>
+__device__ __forceinline__ float parts_max(const DistillArgs& a, uint64_t row) {
+    const float* const parts = a.parts + 2 * row * a.n_chunks;
+    float m = -INFINITY;
+    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) m = fmaxf(m, parts[2 * c]);
+    return m;
+}
+template <int NT>
+__device__ __forceinline__ double parts_sum(const DistillArgs& a, uint64_t row, float ref) {
+    const float* const parts = a.parts + 2 * row * a.n_chunks;
+    double sum = 0.0;
+    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) {
+        const float pm = parts[2 * c];
+        // (a chunk without a number: its sum is 0, or NaN, and stays that)
+        sum += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
+    }
+    return sum;
+}
+
 // a row's chunks joined, and its loss
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
@@ -384,27 +442,17 @@ __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
     const bool lead = (threadIdx.x & 63u) == 0u;
     const uint64_t row = (uint64_t)a.row0 + blockIdx.x;
     const E* const z = reinterpret_cast<const E*>(a.z) + row * a.z_stride;
-    const float* const parts = a.parts + 2 * row * a.n_chunks;
     Teacher<NT> l;
     l.ask(a, row);
     float lt = wave_max(l.template take<T>(a, row, z, 0u, a.n_cols, list));
-    // (a thread's chunks at the thread's own maximum, then to the row's)
-    float m = -INFINITY;
-    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) m = fmaxf(m, parts[2 * c]);
-    m = wave_max(m);
+    float m = wave_max(parts_max<NT>(a, row));
     if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
     const float ref = m == -INFINITY ? 0.0f : m;
-    double sum = 0.0;
-    for (uint32_t c = threadIdx.x; c < a.n_chunks; c += NT) {
-        const float pm = parts[2 * c];
-        // (a chunk without a number: its sum is 0, or NaN, and stays that)
-        sum += (double)parts[2 * c + 1] * (pm == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, pm, ref)));
-    }
     l.sums(a, lt, ref, list);
-    sum = wave_sum(sum);
+    double sum = wave_sum(parts_sum<NT>(a, row, ref));
     l.sum = wave_sum(l.sum);
     l.cross = wave_sum(l.cross);
     if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; meet.sum[2][wid] = l.cross; }
@@ -416,8 +464,9 @@ __global__ void __launch_bounds__(NT) distill_join_kernel(const DistillArgs a) {
     if (threadIdx.x == 0) write_row(a, row, m, sum, l);
 }
 
-// the gradient of one chunk of one row, from the row's saved norm
-template <typename T, int NT>
+// the gradient of one chunk of one row, from the row's saved norm, or (JOIN) from its chunks' parts, joined by every workgroup
+// anew; a row's first chunk then writes the row's loss and norm
+template <typename T, int NT, bool JOIN>
 __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     typedef typename T::elem E;
     constexpr int NW = NT / 64;
@@ -445,22 +494,23 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     if (tail) et = (float)z[ct];
     l.clear(a, list);
     float lt = wave_max(l.template take<T>(a, row, z, c0, c1, list));
-    if (lead) meet.top[1][wid] = lt;
+    float m = JOIN ? wave_max(parts_max<NT>(a, row)) : a.norm_in[2 * row];
+    if (lead) { meet.top[0][wid] = m; meet.top[1][wid] = lt; }
     __syncthreads();   // (everything has been read before anything is overwritten)
 #pragma unroll
-    for (int w = 0; w < NW; ++w) lt = fmaxf(lt, meet.top[1][w]);
+    for (int w = 0; w < NW; ++w) { m = fmaxf(m, meet.top[0][w]); lt = fmaxf(lt, meet.top[1][w]); }
+    const float ref = m == -INFINITY ? 0.0f : m;
     l.enter(a, list, c0, c1);
     l.sums(a, lt, 0.0f, list);
+    double sum = JOIN ? wave_sum(parts_sum<NT>(a, row, ref)) : 0.0;
     l.sum = wave_sum(l.sum);
-    if (lead) meet.sum[1][wid] = l.sum;
+    if (lead) { meet.sum[0][wid] = sum; meet.sum[1][wid] = l.sum; }
     __syncthreads();
-    l.sum = 0.0;
+    sum = l.sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) l.sum += meet.sum[1][w];
+    for (int w = 0; w < NW; ++w) { sum += meet.sum[0][w]; l.sum += meet.sum[1][w]; }
     l.finish();
-    const float m = a.norm_in[2 * row];
-    const float ref = m == -INFINITY ? 0.0f : m;
-    const float per_sum = (float)exp(-(double)a.norm_in[2 * row + 1]);
+    const float per_sum = JOIN ? (float)(1.0 / sum) : (float)exp(-(double)a.norm_in[2 * row + 1]);
     const float gt = a.temperature * (a.weight ? a.weight[row] : 1.0f);
     const float f = gt * per_sum;
 #pragma unroll
@@ -476,6 +526,14 @@ __global__ void __launch_bounds__(NT) distill_grad_kernel(const DistillArgs a) {
     __threadfence_block();
     __syncthreads();
     if (l.some) l.template patch<T>(a, list, g, c0, c1, ref, per_sum, gt);
+    if constexpr (JOIN) {
+        if (c0 == 0 && threadIdx.x == 0) {
+            const float* const from = list_part(a, row);
+            const uint64_t bits = (uint64_t)__builtin_bit_cast(uint32_t, from[0]) | (uint64_t)__builtin_bit_cast(uint32_t, from[1]) << 32;
+            l.cross = __builtin_bit_cast(double, bits) - ((double)from[2] - (double)ref) * l.sum;
+            write_row(a, row, m, sum, l);
+        }
+    }
 }
 
 // One workgroup a row, or a chunk of one, and a launch for every 2^20 of them (a kernel without a loop over rows keeps nothing
@@ -511,10 +569,10 @@ void launch_row(const DistillArgs& args, hipStream_t st) {
     });
 }
 
-template <typename T>
+template <typename T, bool JOIN>
 void launch_grad(const DistillArgs& args, hipStream_t st) {
     for_rows(args, args.n_chunks, [&](const DistillArgs& a, dim3 grid) {
-        hipLaunchKernelGGL((distill_grad_kernel<T, 256>), grid, dim3(256), list_bytes(a, true), st, a);
+        hipLaunchKernelGGL((distill_grad_kernel<T, 256, JOIN>), grid, dim3(256), list_bytes(a, true), st, a);
     });
 }
 
@@ -543,18 +601,26 @@ void launch_loss(DistillArgs a, hipStream_t st) {
         else launch_row<T, 512, 16>(a, st);
         return;
     }
-    for_rows(a, a.n_chunks, [&](const DistillArgs& a, dim3 grid) { hipLaunchKernelGGL((distill_part_kernel<T, 256>), grid, dim3(256), 0, st, a); });
+    // Parts and gradient, whose workgroups join the parts in passing while there are few of them (us: 9 x 686339 bf16 16.8, with a
+    // launch for the joining 18.9; 64 x 300000 27.7, 30.6; 1000 x 152064 189, 193; 1000 parts a row take the same time either way).
+    if (a.grad && a.n_chunks <= JOIN_MAX) {
+        for_rows(a, a.n_chunks, [&](const DistillArgs& a, dim3 grid) {
+            hipLaunchKernelGGL((distill_part_kernel<T, 256, true>), grid, dim3(256), list_bytes(a, false), st, a);
+        });
+        return launch_grad<T, true>(a, st);
+    }
+    for_rows(a, a.n_chunks, [&](const DistillArgs& a, dim3 grid) { hipLaunchKernelGGL((distill_part_kernel<T, 256, false>), grid, dim3(256), 0, st, a); });
     for_rows(a, 1, [&](const DistillArgs& a, dim3 grid) { hipLaunchKernelGGL((distill_join_kernel<T, 256>), grid, dim3(256), list_bytes(a, false), st, a); });
     if (a.grad) {
         a.norm_in = a.norm;
-        launch_grad<T>(a, st);
+        launch_grad<T, false>(a, st);
     }
 }
 
 uint64_t work_bytes(uint32_t n_rows, uint32_t n_cols) {
     if (n_cols <= ROW_MAX || n_rows == 0) return 0;
     const uint32_t chunk = chunk_of(n_rows, n_cols);
-    return (uint64_t)n_rows * (((uint64_t)n_cols + chunk - 1) / chunk) * 2u * sizeof(float);
+    return (uint64_t)n_rows * ((((uint64_t)n_cols + chunk - 1) / chunk) * 2u + 3u) * sizeof(float);
 }
 
 trag_status check_distill(const std::string& who, const DistillArgs& a, uint32_t dtype) {
@@ -641,9 +707,9 @@ trag_status trag_distill_grad_device(const void* d_logits, uint64_t logits_strid
         OpDevice on(who, hip_stream, {d_logits, d_ids, d_teacher, d_counts, d_norm, d_row_weight, d_grad});
         if (on.status != TRAG_OK) return on.status;
         const hipStream_t st = (hipStream_t)hip_stream;
-        if (dtype == TRAG_F32) launch_grad<F32by8>(a, st);
-        else if (dtype == TRAG_F16) launch_grad<F16>(a, st);
-        else launch_grad<BF16>(a, st);
+        if (dtype == TRAG_F32) launch_grad<F32by8, false>(a, st);
+        else if (dtype == TRAG_F16) launch_grad<F16, false>(a, st);
+        else launch_grad<BF16, false>(a, st);
         return op_launched(who);
     });
 }
