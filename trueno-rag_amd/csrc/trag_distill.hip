@@ -48,7 +48,7 @@ struct DistillArgs {
     const float* norm_in;     // the same, for the gradient alone
     const float* weight;      // per row, null: 1
     void* grad;
-    float* parts;             // 2 per row and chunk, behind them 3 per row (list_part)
+    float* parts;             // 2 per row and chunk, behind them 4 per row (list_part)
     uint64_t z_stride, grad_stride;
     uint32_t n_rows, n_cols, k, chunk, n_chunks;
     uint32_t row0;            // first row of a launch
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(NT, NT == 512 && sizeof(typename T::elem) == 2
 
 // What a row's list comes to before the row's maximum is known, behind the parts: a double, the sum of
 // e ((t - max t) - (z_id - zl)), and zl, the list's largest logit -- differences of logits, which lose nothing where the logits are huge.
-__device__ __forceinline__ float* list_part(const DistillArgs& a, uint64_t row) { return a.parts + 2 * (uint64_t)a.n_rows * a.n_chunks + 3 * row; }
+__device__ __forceinline__ float* list_part(const DistillArgs& a, uint64_t row) { return a.parts + 2 * (uint64_t)a.n_rows * a.n_chunks + 4 * row; }
 
 // (max, sum) of one chunk of one row; a chunk is at most PART_VECS vectors a thread. LIST: a row's first chunk does the list's
 // part of the loss too, while the logits are what they were (a gradient may go in their place).
@@ -620,7 +620,7 @@ void launch_loss(DistillArgs a, hipStream_t st) {
 uint64_t work_bytes(uint32_t n_rows, uint32_t n_cols) {
     if (n_cols <= ROW_MAX || n_rows == 0) return 0;
     const uint32_t chunk = chunk_of(n_rows, n_cols);
-    return (uint64_t)n_rows * ((((uint64_t)n_cols + chunk - 1) / chunk) * 2u + 3u) * sizeof(float);
+    return (uint64_t)n_rows * ((((uint64_t)n_cols + chunk - 1) / chunk) * 2u + 4u) * sizeof(float);
 }
 
 trag_status check_distill(const std::string& who, const DistillArgs& a, uint32_t dtype) {
