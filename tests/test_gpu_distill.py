@@ -157,9 +157,9 @@ def test_loss_and_gradient_match_the_formula(trag, t, cols):
 
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,cols", [(1100, 1900), (1025, 4001), (2561, 25003), (2 ** 20 + 77, 5)])
+@pytest.mark.parametrize("rows,cols", [(1100, 1900), (1025, 4001), (2561, 25003), (2 ** 20 + 77, 5), (1, 2_200_003), (3, 700_001)])
 def test_many_rows(trag, t, rows, cols):
-    """The forms for many rows, and more rows than one launch takes."""
+    """The forms for many rows, more rows than one launch takes, and rows of more parts than the gradient joins."""
     torch = _torch()
     z0, ids, teacher, counts, weight = _case(rows, cols, 4, cols)
     zb, z = _filled(z0, _types()[t], 1, 1)
