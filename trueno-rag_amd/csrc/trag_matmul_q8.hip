@@ -526,7 +526,7 @@ bool dma_fits(const MmArgs& p) {
 //   4096 x 16384 x 4096  256 x 256  235    128 x 128 in 1  290
 //   1 x 1M x 384  16 x 64 in 1  66    64 x 1M x 384  64 x 128  102, 64 x 64  108    128 x 1M x 384  128 x 128  136, 64 x 64  180
 // and for rows at any byte (through registers):
-//   3 x 887 x 4404  16 x 16 in 8  5.2, 32 x 64 in 4  8.7    37 x 50021 x 777  64 x 128  12.2, 64 x 64  13.5
+//   15 x 2154 x 7715  16 x 16 in 8  9.5, 16 x 32 in 4  12.8, 32 x 64 in 4  21.9    37 x 50021 x 777  64 x 128  12.2, 64 x 64  13.5
 //   512 x 4096 x 4001  64 x 64  22.6, 64 x 128  23.0, 128 x 128  28.8    4096 x 8192 x 4001  256 x 256  150, 128 x 128  189
 enum TileForm { T16x16G8, T16x32G4, T16, T16G4, T32, T32G4, T64, T64G2, T64x128, T128, T128G2, T256, N_FORMS };
 struct FormCost {
