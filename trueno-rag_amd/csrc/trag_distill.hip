@@ -187,18 +187,22 @@ struct Teacher {
     template <typename T>
     __device__ __forceinline__ void patch(const DistillArgs& a, const List& l, typename T::elem* g, uint32_t c0, uint32_t c1,
                                           float ref, float per_sum, float gt) const {
-        const float inv = (float)(1.0 / sum);
+        const double inv64 = 1.0 / sum;
+        const float inv = (float)inv64;
         for (uint32_t j = threadIdx.x; j < a.k; j += NT) {
             const uint32_t id = l.id[j];
             if (id == NO_ID || id < c0 || id >= c1) continue;
             uint32_t s = home(a, id);
             while (l.slot_id[s] != id) s = (s + 1u) & a.slot_mask;   // (it has been entered)
             if (l.slot_first[s] != j) continue;
-            float e = l.e[j];
-            if (l.slot_again[s >> 5] >> (s & 31u) & 1u)
+            float p = l.e[j] * inv;
+            if (l.slot_again[s >> 5] >> (s & 31u) & 1u) {   // (up to 1024 terms: in 32 bits they lost up to 25 * 2^-24)
+                double e = (double)l.e[j];
 #pragma unroll 8
-                for (uint32_t o = j + 1u; o < a.k; ++o) e += l.id[o] == id ? l.e[o] : 0.0f;
-            g[id] = T::round(gt * (exp2_hw(expo(a, l.z[j], ref)) * per_sum - e * inv));
+                for (uint32_t o = j + 1u; o < a.k; ++o) e += l.id[o] == id ? (double)l.e[o] : 0.0;
+                p = (float)(e * inv64);
+            }
+            g[id] = T::round(gt * (exp2_hw(expo(a, l.z[j], ref)) * per_sum - p));
         }
     }
 
