@@ -556,7 +556,7 @@ trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const fl
 /* Distillation from a teacher's best k. Row r of the teacher is the list of the first
  * min(d_counts[r], k) pairs at r * k of d_ids (columns) and d_teacher (scores); d_counts NULL: all k. An
  * id of n_cols or more marks an absent entry (it is left out, as if its score were minus infinity). The
- * same id may stand in a list more than once; its probabilities add up. With T = temperature,
+ * same id may stand in a list more than once; its probabilities add up. With T = temperature (5e-39 to 1e36),
  *   p = softmax(teacher / T) over the list,  q = softmax(logits / T) over the row,
  *   loss[r] = T^2 * sum_j p_j (log p_j - log q[id_j]),
  *   grad[r][c] = row_weight[r] * T * (q_c - sum of p_j with id_j = c).

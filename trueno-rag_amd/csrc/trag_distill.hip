@@ -632,9 +632,10 @@ trag_status check_distill(const std::string& who, const DistillArgs& a, uint32_t
     if (dtype > TRAG_BF16) return bad("unknown element type");
     if (a.n_cols == 0) return bad("rows of 0 columns");
     if (!a.z || (a.k && (!a.ids || !a.teacher))) return bad("null array");
-    // (and its reciprocal finite in 32 bits, which leaves out temperatures below 5e-39)
-    if (!(a.temperature > 0.0f) || !(a.temperature - a.temperature == 0.0f) || !(a.c - a.c == 0.0f))
-        return bad("the temperature must be positive and finite");
+    // (and its reciprocal finite in 32 bits, which leaves out temperatures below 5e-39; a difference of two logits is an infinity in
+    // 32 bits from 3.4e38 on, whose exponential over a temperature of 1e36 is 0 as it should be, and over 1e38 e^-3.4)
+    if (!(a.temperature > 0.0f) || !(a.temperature <= 1e36f) || !(a.c - a.c == 0.0f))
+        return bad("the temperature must be positive, and neither below 5e-39 nor above 1e36");
     const uint32_t e = dtype_bytes(dtype);
     if (!aligned_to(a.z, e) || !aligned_to(a.grad, e) || !aligned_to(a.ids, 4) || !aligned_to(a.teacher, 4) ||
         !aligned_to(a.counts, 4) || !aligned_to(a.loss, 4) || !aligned_to(a.norm, 4) || !aligned_to(a.norm_in, 4) ||
