@@ -256,6 +256,8 @@ class VectorStore:
     def quantize_device(self, row0: int, n: int, q8_ptr: int, q8_stride: int, scale_ptr: int, stream: int = 0) -> None:
         """Rows [row0, row0 + n) as 8-bit integers with a scale each, written to device arrays: the corpus
         operand of q8.matmul_q8_device (trag_store_quantize_device)."""
+        if n >> 32:
+            raise _abi.TragError(_abi.INVALID_ARG, "a count does not fit 32 bits")
         _abi.check(_abi.lib().trag_store_quantize_device(self._h, row0, n, q8_ptr, q8_stride, scale_ptr, stream))
 
     def _id_for_row(self, row: int) -> ChunkId:
