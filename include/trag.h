@@ -517,7 +517,8 @@ trag_status trag_bm25_stats(trag_bm25 *ix, uint64_t *postings, uint64_t *terms);
  * graph and called by several threads. Strides count elements from row to row; rows may start at any
  * element (16-byte alignment is not needed, and only the product goes faster with it). A call of 0
  * rows is TRAG_OK and touches nothing; rows of 0 elements are TRAG_INVALID_ARG. Outputs must not overlap
- * inputs, except where said.
+ * inputs, except where said. An error that an earlier HIP call of the program left in the runtime's record
+ * (hipGetLastError) does not fail the call: it is cleared, and trag_last_error() names it.
  * ------------------------------------------------------------------------ */
 typedef enum trag_dtype { TRAG_F32 = 0, TRAG_F16 = 1, TRAG_BF16 = 2 } trag_dtype;
 

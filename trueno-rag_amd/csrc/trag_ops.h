@@ -90,8 +90,11 @@ struct OpDevice {
             }
         }
         if (dev >= 0 && hipGetDevice(&prev) == hipSuccess && prev != dev) switched = hipSetDevice(dev) == hipSuccess;
-        // (an error that a call of the program's before this one has left behind: op_launched would take it for the launch's)
-        (void)hipGetLastError();
+        // (an error that a call of the program's before this one has left behind: op_launched would take it for the launch's; the
+        // runtime's record of it cannot be put back, so the message says what it was)
+        const hipError_t left = hipGetLastError();
+        if (left != hipSuccess)
+            (void)set_error(TRAG_OK, std::string(who) + ": an earlier HIP call of the program had failed (" + hipGetErrorString(left) + "); its error is cleared");
     }
     ~OpDevice() {
         if (switched) (void)hipSetDevice(prev);
