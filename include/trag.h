@@ -562,7 +562,9 @@ trag_status trag_matmul_q8_device(const int8_t *d_a, uint64_t a_stride, const fl
  *   loss[r] = T^2 * sum_j p_j (log p_j - log q[id_j]),
  *   grad[r][c] = row_weight[r] * T * (q_c - sum of p_j with id_j = c).
  * A row whose list is empty (or all minus infinity) is left out: loss 0 and gradient 0, whatever its
- * logits. d_norm receives two floats a row, max(logits) and log sum exp((logits - max) / T): what
+ * logits. In any other row a logit or a score that is NaN or plus infinity makes the loss NaN, logits that are
+ * minus infinity throughout loss and gradient; a column with probability at minus infinity makes the loss
+ * infinite. d_norm receives two floats a row, max(logits) and log sum exp((logits - max) / T): what
  * trag_distill_grad_device needs. d_grad NULL: the loss alone; otherwise the gradient too, in the
  * logits' type, for row weights known beforehand (d_row_weight, NULL: ones). d_grad may be d_logits
  * itself, with its stride. d_work: trag_distill_work_bytes(n_rows, n_cols) bytes, 4-byte aligned, in use
