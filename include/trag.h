@@ -507,7 +507,7 @@ trag_status trag_bm25_stats(trag_bm25 *ix, uint64_t *postings, uint64_t *terms);
  * serve are those of VectorStore::search (src/index.rs:386-412). An encoder's hidden states become
  * rows of 8-bit integers with one scale a row (trag_rmsnorm_q8_device), a corpus does so directly
  * (trag_quantize_q8_device, trag_store_quantize_device), their product gives every score
- * (trag_matmul_q8_device), and the lists of trag_store_search_device -- ids, scores and counts, as they
+ * (trag_matmul_q8_device; picking the best of them is the caller's), and the lists of trag_store_search_device -- ids, scores and counts, as they
  * are in device memory -- are the teacher of the loss (trag_distill_loss_device).
  *
  * All pointers are device pointers; work is enqueued on hip_stream and the call returns at once. The

@@ -9,11 +9,14 @@
 // gradient needs the row again. Bound by HBM: one read of the logits for the loss, one read and one write
 // for a gradient. Rows of up to 65536 columns stay in registers between the sum and the gradient; longer rows
 // are cut into chunks, each in the registers of one workgroup, whose partial (m, sum) pairs are joined by a second
-// launch, the gradient's where there is one, which reads the logits again.
+// launch, the gradient's where there is one, which reads the logits again; a gradient over more than 1024 chunks a row
+// takes three (parts, joining, gradient).
 //
 // Exponentials go through exp2 of (z - m) log2(e) / T: the difference first, so that rows at the type's lowest
 // value, whose product with 1 / T would overflow, still come out as the distribution they are. Sums over a
-// row are 32-bit per thread and chunk, 64-bit across them; the k terms of the loss are 64-bit.
+// row are 32-bit per thread, 64-bit across threads, and a chunk's is rounded to 32 bits once more where it goes to memory: 24 or
+// 34 roundings of 2^-24 a row, beside the exponentials' own. The teacher's exponentials are 32-bit (3 * 2^-24, the hardware's
+// exp2), their sums, over a repeated id too, and the differences of logits they weight 64-bit.
 #include <algorithm>
 #include "trag_ops.h"
 
@@ -247,8 +250,9 @@ __device__ __forceinline__ void keep_raw(typename T::vec (&h)[NV]) {
 
 // One workgroup a row, the row in registers as NV vectors of W columns a thread (the columns behind the last
 // whole vector: one each for the first few threads): one read of the logits, one write of the gradient, two meetings
-// of the waves and one more before the list's columns are set right. (Sixteen vectors of eight waves are held to 128 registers, so
-// that two rows fit a CU: 1000 x 50257 bf16 with the gradient 58 us, with one row a CU 71.)
+// of the waves and one more before the list's columns are set right. (Sixteen 16-bit vectors of eight waves are held to 128
+// registers, so that two rows fit a CU: 1000 x 50257 bf16 with the gradient 60 us. Without the bound they take 134, one row a CU, 67
+// us; the bound costs six registers, 28 bytes of scratch a thread. With a loop over rows they took 194, 72 us.)
 template <typename T, int NT, int NV, bool GRAD>
 __global__ void __launch_bounds__(NT, NT == 512 && sizeof(typename T::elem) == 2 ? 4 : 1) distill_row_kernel(const DistillArgs a) {
     typedef typename T::elem E;
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(NT) distill_part_kernel(const DistillArgs a) {
         for (int w = 0; w < NW; ++w)   // (a wave without a number: its sum is 0, or NaN, and stays that)
             sum += meet.sum[0][w] * (meet.top[0][w] == -INFINITY ? 1.0 : (double)exp2_hw(expo(a, meet.top[0][w], top)));
         a.parts[2 * part] = top;
-        a.parts[2 * part + 1] = (float)sum;
+        a.parts[2 * part + 1] = (float)sum;   // (one rounding beside the 33 of a thread's own sum; the pair stays 8 bytes)
     }
 }
 
@@ -595,13 +599,15 @@ template <typename T>
 void launch_loss(DistillArgs a, hipStream_t st) {
     if (a.n_cols <= ROW_MAX) {
         // The fewest threads that hold the row, where there are rows enough to fill the chip (with the gradient, us: 5000 x 2000 bf16
-        // one wave a row 15.8, two 16.9, four 20.4; 5000 x 4000 two waves 23.3, one 23.4, four 26.1, f32 43.8, 46.0, 41.0; 5000 x
-        // 8000 bf16 four waves 37.6, two 43.6, eight 45.8; 4096 x 20000 four waves 69, eight 79); few rows of two vectors a thread
-        // (64 x 4000 four waves 6.6, two 6.9, one 7.9).
+        // one wave a row 15.8, two 16.9, four 20.4; 5000 x 4000 two waves 23.3, one 23.4, four 26.1; 5000 x 8000 four waves 37.6, two
+        // 43.6, eight 45.8; 4096 x 20000 four waves 69, eight 79); few rows of two vectors a thread (64 x 4000 four waves 6.6, two
+        // 6.9, one 7.9). The types share the rule, which costs f32 7 % at 5000 x 4000 (two waves 43.8, four 41.0), and it stops short of
+        // eight waves for rows of 8193 to 32768 columns, which are faster where there are few (1 x 30000 8.7 us, eight waves 7.8; 64 x 30000
+        // 9.6, 8.6; 300 x 16000 10.5, 10.2; 2000 x 16000 the same) and at 5000 x 16000 (72, 66).
         const bool many = a.n_rows >= 1024u;
         // (Very many rows of nearly what four waves hold: as 16-bit rows of eight waves three of them are on a CU at a time instead of
         // four, and reads and writes get in each other's way less. 4096 x 32000 bf16 with the gradient 104 us, four waves 111;
-        // 8192 x 32000 191, 215; but 2000 x 29999 64, 60 and 4096 x 20000 79, 69.)
+        // 8192 x 32000 191, 215; but 2000 x 29999 64, 60 and 4096 x 20000 79, 69. Both bounds lie between measured sizes.)
         if constexpr (sizeof(typename T::elem) == 2)
             if (a.n_cols > 24576u && a.n_cols <= 32768u && a.n_rows >= 2560u) return launch_row<T, 512, 8>(a, st);
         if (a.n_cols <= 512u) launch_row<T, 64, 1>(a, st);

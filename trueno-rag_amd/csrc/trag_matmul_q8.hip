@@ -185,10 +185,14 @@ __global__ void __launch_bounds__(64 * WK * WN) mm_direct_kernel(const MmArgs p)
 // way; the permutation is applied to the addresses that the lanes fetch), ST stages deep. Otherwise the same through
 // registers, two stages.
 // KG: groups of waves that share a tile's terms, each with stages of its own, where there are few tiles.
-// What bounds it (4096 x 16384 x 4096, 236 us, 2.33 POP/s; 8192 x 8192 x 8192 440 us, 2.50): the matrix cores at the 2.0 GHz
-// that they hold under this load are half busy, fragment reads 22 % of LDS's cycles; reading fragments ahead of the
-// multiplications (128 x 128 tiles 355 -> 303 us) and moving the transfers within a step do not change the largest tile's time.
-// A plain large 8-bit library product takes 288 and 527 us for the two.
+// What bounds it (4096 x 16384 x 4096, 237 to 245 us from card to card, 2.3 POP/s; 8192 x 8192 x 8192 437 us, 2.5): the matrix cores
+// at the 1.9 to 2.0 GHz that they hold under this load are busy 58 % of the cycles, LDS 25 %, bank conflicts 1.4 % among them;
+// reading fragments ahead of the multiplications (128 x 128 tiles 355 -> 303 us) and moving the transfers within a step do not
+// change the largest tile's time. A plain large 8-bit library product takes 288 and 527 us for the two.
+// Where the terms are few or the tiles do not fill the CUs the time is 1.6 to 2.3 times that of the traffic or of the matrix cores:
+// 4096 x 16384 x 384 bf16 65 us of 27, f32 93 of 53, 1000 x 50000 x 384 f32 70 of 42, 315 x 7024 x 7936 39 of 17. A 256 x 256
+// tile of 384 terms is three steps and 4.9 us of filling stages and epilogue with nothing beside it on the CU; 165 tiles of 128 x 128 are
+// fewer than the CUs.
 template <typename T, int WM, int WN, int MT, int NT, int KG, int ST, bool DMA>
 __global__ void __launch_bounds__(64 * WM * WN * KG, 2) mm_tile_kernel(const MmArgs p) {
     typedef typename T::elem E;
@@ -517,7 +521,7 @@ bool dma_fits(const MmArgs& p) {
 // rounds = tiles over what 256 CUs work on at once; `per`, the time of a 128-byte step, grows from `lo` to `hi` as the CUs fill
 // up (12 TB/s for rows at any byte). The constants are fitted, form by form, to the times of 1900 products of random sizes
 // (1 to 4096 by 64 to 1M by 32 to 8192); over 1000 others the choice takes 1.8 % longer than the best form on average, 11 % in
-// the worst twentieth. Some of the times (us of the kernel among others of its kind; bf16 output; aligned rows, m x n x dim):
+// the worst twentieth (against the best form, not against what the traffic allows). Some of the times (us of the kernel among others of its kind; bf16 output; aligned rows, m x n x dim):
 //   16 x 4096 x 4096   16 x 16 tiles in 8 groups of waves  6.3    16 x 32 in 4  6.4    16 x 64 in 4  7.5    in 1  16.6
 //   8 x 2048 x 8192    16 x 16 in 8   6.4    16 x 32 in 4   8.2    16 x 64 in 4  10.5    in 1  30.3
 //   100 x 1000 x 4096  16 x 32 in 4   6.2    16 x 64 in 4   7.4    32 x 64 in 4   8.3    16 x 16 in 8   8.4

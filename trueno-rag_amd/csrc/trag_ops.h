@@ -1,6 +1,6 @@
 // What the operators on a caller's device arrays share (trag_q8.hip, trag_matmul_q8.hip,
-// trag_distill.hip): element types, eight elements at a time, workgroup reductions, and the checks
-// of an entry point that has no handle to ask for its device.
+// trag_distill.hip): element types, 16 bytes of them at a time, and the checks of an entry point that
+// has no handle to ask for its device.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdint>
